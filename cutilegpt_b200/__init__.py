@@ -15,6 +15,9 @@ from .kernels import (
     cutile_layer_norm,
     cutile_causal_attention,
     cutile_fused_mlp,
+    PagedKV,
+    cutile_paged_kv_append,
+    cutile_shared_prefix_attention,
 )
 from .api import (
     TileOp,
@@ -49,4 +52,7 @@ __all__ = [
     'cutile_layer_norm',
     'cutile_causal_attention',
     'cutile_fused_mlp',
+    'PagedKV',
+    'cutile_paged_kv_append',
+    'cutile_shared_prefix_attention',
 ]

@@ -42,6 +42,19 @@ class GemmFusion(ctypes.Structure):
     ]
 
 
+class PagedKvStruct(ctypes.Structure):
+    """struct gpt_paged_kv (include/gpt_b200.h): a paged key/value cache and its tables."""
+    _fields_ = [
+        ("k_pages", _p), ("v_pages", _p), ("n_pages", _i64), ("page_size", _i64), ("kv_heads", _i64),
+        ("head_dim", _i64), ("page_stride", _i64), ("head_stride", _i64), ("slot_stride", _i64),
+        ("page_table", _p), ("ld_page_table", _i64), ("max_pages", _i64), ("seq_lens", _p), ("batch", _i64),
+        ("prefix_table", _p), ("ld_prefix_table", _i64), ("max_prefix_pages", _i64), ("prefix_lens", _p),
+        ("n_groups", _i64),
+    ]
+
+
+_pkv = ctypes.POINTER(PagedKvStruct)
+
 # name -> (restype, argtypes); mirrors include/gpt_b200.h
 SIGNATURES = {
     "gpt_version": (_i32, []),
@@ -71,6 +84,10 @@ SIGNATURES = {
                               ctypes.POINTER(GemmFusion), _i32, _p]),
     "gpt_row_stats": (_i32, [_p, _i64, _i64, _i64, _p, _i32, _p]),
     "gpt_row_sums": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i32, _p]),
+    "gpt_paged_kv_append": (_i32, [_p, _pi64, _p, _pi64, _p, _pi64, _p, _pi64, _i64, _i64, _pkv, _p, _i64, _i64, _i32,
+                                   _i32, _p]),
+    "gpt_attention_shared_prefix_workspace_size": (_i64, [_i64, _i64, _pkv, _i32]),
+    "gpt_attention_shared_prefix": (_i32, [_p, _pi64, _p, _pi64, _i64, _i64, _pkv, _f32, _p, _i64, _i32, _p]),
     "gpt_lnfold_weights": (_i32, [_p, _p, _p, _p, _i64, _i64, _p, _p, _p, _i32, _p]),
 }
 

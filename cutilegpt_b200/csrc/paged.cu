@@ -1,0 +1,235 @@
+// C entry points of the paged key/value cache and the plan of an attention
+// call: which kernels run, over how many shares of the keys.
+#include <math.h>
+
+#include "paged.cuh"
+
+namespace gpt {
+namespace paged {
+
+// Checks what both operators need of a cache description.
+static int check_kv(const gpt_paged_kv* kv, const char* what) {
+  GPT_CHECK_ARG(kv, "%s: null cache description", what);
+  GPT_CHECK_SHAPE(kv->batch >= 0 && kv->batch < (1LL << 24) && kv->kv_heads > 0 && kv->kv_heads < (1 << 20) &&
+                      kv->head_dim > 0 && kv->head_dim <= 256,
+                  "%s: bad sizes batch=%lld kv_heads=%lld head_dim=%lld (1..256)", what, (long long)kv->batch,
+                  (long long)kv->kv_heads, (long long)kv->head_dim);
+  GPT_CHECK_SHAPE(kv->n_pages > 0 && kv->n_pages < (1LL << 31) && kv->page_size > 0 && kv->page_size < (1LL << 30),
+                  "%s: bad sizes n_pages=%lld page_size=%lld", what, (long long)kv->n_pages, (long long)kv->page_size);
+  GPT_CHECK_SHAPE(kv->page_stride >= 0 && kv->head_stride >= 0 && kv->slot_stride >= 0,
+                  "%s: negative cache stride", what);
+  GPT_CHECK_SHAPE(kv->max_pages > 0 && kv->max_pages <= (1LL << 30) / kv->page_size &&
+                      kv->ld_page_table >= kv->max_pages,
+                  "%s: page_table rows list %lld pages (row stride %lld) of %lld positions; a row lists 1 to 2^30 positions",
+                  what, (long long)kv->max_pages, (long long)kv->ld_page_table, (long long)kv->page_size);
+  GPT_CHECK_SHAPE(kv->n_groups >= 0 && (kv->n_groups == 0 || kv->batch % kv->n_groups == 0),
+                  "%s: n_groups=%lld does not divide batch=%lld", what, (long long)kv->n_groups, (long long)kv->batch);
+  if (kv->n_groups > 0)
+    GPT_CHECK_SHAPE(kv->max_prefix_pages > 0 && kv->max_prefix_pages <= (1LL << 30) / kv->page_size &&
+                        kv->ld_prefix_table >= kv->max_prefix_pages,
+                    "%s: prefix_table rows list %lld pages (row stride %lld) of %lld positions; a row lists 1 to 2^30 positions",
+                    what, (long long)kv->max_prefix_pages, (long long)kv->ld_prefix_table, (long long)kv->page_size);
+  return GPT_OK;
+}
+
+static int check_kv_pointers(const gpt_paged_kv* kv, const char* what) {
+  GPT_CHECK_ARG(kv->k_pages && kv->v_pages && kv->page_table && kv->seq_lens, "%s: null cache pointer", what);
+  GPT_CHECK_ARG(kv->n_groups == 0 || (kv->prefix_table && kv->prefix_lens), "%s: null prefix pointer", what);
+  return GPT_OK;
+}
+
+// How an attention call runs.
+struct Plan {
+  int shared;          // the prefix apart from the own positions, once for a group
+  int n_pre, n_own;    // shares of the keys with partial results of their own; n_own = 1: the last launch writes out
+  int64_t bytes;       // workspace
+};
+
+// Shares of `keys` keys for `items` CTAs of equal work: enough for two CTAs on every SM, at
+// least 128 keys in a share.
+static int shares(int64_t items, int64_t keys, int sms) {
+  const int64_t want = (2 * (int64_t)sms + items - 1) / (items > 0 ? items : 1);
+  const int64_t most = (keys + 127) / 128;
+  const int64_t s = want < most ? want : most;
+  return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+}
+
+static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv) {
+  int sms = device_sm_count();
+  if (sms <= 0) sms = 148;
+  Plan pl = {};
+  const int64_t groups = kv->n_groups, per = groups > 0 ? kv->batch / groups : kv->batch;
+  const int64_t share = H / kv->kv_heads, own_keys = kv->max_pages * kv->page_size;
+  const int64_t pre_keys = groups > 0 ? kv->max_prefix_pages * kv->page_size : 0;
+  pl.shared = groups > 0 && per > 1;
+  const int64_t own_blocks = (T * share + 15) / 16, pre_blocks = (per * T * share + 15) / 16;
+  if (pl.shared) {
+    pl.n_pre = shares(groups * kv->kv_heads * pre_blocks, pre_keys, sms);
+    pl.n_own = shares(kv->batch * kv->kv_heads * own_blocks, own_keys, sms);
+  } else {
+    pl.n_own = shares(kv->batch * kv->kv_heads * own_blocks, own_keys + pre_keys, sms);
+  }
+  const int64_t slots = pl.n_pre + (pl.n_own > 1 ? pl.n_own : 0);
+  pl.bytes = slots * kv->batch * T * H * (kv->head_dim + 2) * (int64_t)sizeof(float);
+  return pl;
+}
+
+template <typename T>
+static int run(Attn& p, const Plan& pl, cudaStream_t st) {
+  p.n_pre = pl.n_pre;
+  p.n_own = pl.n_own > 1 ? pl.n_own : 0;
+  int s = GPT_OK;
+  if (pl.shared) s = launch_simt<T>(p, kPrefix, pl.n_pre, 0, 0, st);
+  if (!s) s = launch_simt<T>(p, pl.shared ? kOwn : kAll, pl.n_own, pl.n_pre, pl.n_own == 1, st);
+  if (!s && pl.n_own > 1) s = launch_join<T>(p, st);
+  return s;
+}
+
+}  // namespace paged
+}  // namespace gpt
+
+extern "C" {
+
+int gpt_paged_kv_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, void* q_out, const int64_t* q_out_strides, int64_t T, int64_t H,
+                        const gpt_paged_kv* kv, const float* cos_sin, int64_t n_pos, int64_t rot, int interleaved,
+                        int dtype, void* stream) {
+  const char* what = "gpt_paged_kv_append";
+  GPT_CHECK_DTYPE(dtype);
+  int s = gpt::paged::check_kv(kv, what);
+  if (s) return s;
+  GPT_CHECK_SHAPE(T >= 0 && T < (1LL << 30) && H > 0 && H < (1 << 20), "%s: bad sizes T=%lld H=%lld", what, (long long)T,
+                  (long long)H);
+  GPT_CHECK_SHAPE(rot >= 0 && rot % 2 == 0 && rot <= kv->head_dim, "%s: rot=%lld must be even and at most head_dim=%lld",
+                  what, (long long)rot, (long long)kv->head_dim);
+  GPT_CHECK_SHAPE(rot == 0 || n_pos > 0, "%s: rotation needs a table of at least one position", what);
+  if (kv->batch == 0 || T == 0) return GPT_OK;
+  s = gpt::paged::check_kv_pointers(kv, what);
+  if (s) return s;
+  GPT_CHECK_ARG(k && v && k_strides && v_strides, "%s: null pointer", what);
+  GPT_CHECK_ARG(rot == 0 || (q && q_out && q_strides && q_out_strides && cos_sin), "%s: rotation needs q, q_out and cos_sin",
+                what);
+  gpt::paged::Append p = {};
+  const size_t es = dtype == GPT_F32 ? 4 : 2;
+  bool wide = kv->head_dim * es % 16 == 0 && gpt::aligned(k, 16) && gpt::aligned(v, 16) && gpt::aligned(kv->k_pages, 16) &&
+              gpt::aligned(kv->v_pages, 16) && kv->page_stride * es % 16 == 0 && kv->head_stride * es % 16 == 0 &&
+              kv->slot_stride * es % 16 == 0;
+  for (int i = 0; i < 3; ++i) {
+    p.k_s[i] = k_strides[i];
+    p.v_s[i] = v_strides[i];
+    wide = wide && k_strides[i] * (int64_t)es % 16 == 0 && v_strides[i] * (int64_t)es % 16 == 0;
+    if (rot) {
+      p.q_s[i] = q_strides[i];
+      p.o_s[i] = q_out_strides[i];
+      wide = wide && q_strides[i] * (int64_t)es % 16 == 0 && q_out_strides[i] * (int64_t)es % 16 == 0;
+    }
+  }
+  if (rot) {
+    // the members of a pair in vectors of their own, or pairs inside a vector
+    wide = wide && gpt::aligned(q, 16) && gpt::aligned(q_out, 16) && gpt::aligned(cos_sin, 16) &&
+           (interleaved ? rot : rot / 2) * es % 16 == 0 && rot % 8 == 0;
+  }
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.q_out = q_out;
+  p.k_pages = kv->k_pages;
+  p.v_pages = kv->v_pages;
+  p.page_stride = kv->page_stride;
+  p.head_stride = kv->head_stride;
+  p.slot_stride = kv->slot_stride;
+  p.n_pages = (int)kv->n_pages;
+  p.page = (int)kv->page_size;
+  p.table = kv->page_table;
+  p.ld_table = kv->ld_page_table;
+  p.cap = (int)(kv->max_pages * kv->page_size);
+  p.seq_lens = kv->seq_lens;
+  p.plens = kv->n_groups > 0 ? kv->prefix_lens : nullptr;
+  p.pcap = kv->n_groups > 0 ? (int)(kv->max_prefix_pages * kv->page_size) : 0;
+  p.per = (int)(kv->n_groups > 0 ? kv->batch / kv->n_groups : kv->batch);
+  p.cos_sin = cos_sin;
+  p.n_pos = n_pos;
+  p.rot = (int)rot;
+  p.interleaved = interleaved != 0;
+  p.T = (int)T;
+  p.K = (int)kv->kv_heads;
+  p.D = (int)kv->head_dim;
+  p.heads = (int)(2 * kv->kv_heads + (rot ? H : 0));
+  const int64_t tokens = kv->batch * T;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == GPT_BF16)
+    return wide ? gpt::paged::launch_append<__nv_bfloat16, 8>(p, tokens, st)
+                : gpt::paged::launch_append<__nv_bfloat16, 1>(p, tokens, st);
+  return wide ? gpt::paged::launch_append<float, 4>(p, tokens, st) : gpt::paged::launch_append<float, 1>(p, tokens, st);
+}
+
+int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H, const gpt_paged_kv* kv, int dtype) {
+  if (gpt::paged::check_kv(kv, "gpt_attention_shared_prefix_workspace_size") || (dtype != GPT_F32 && dtype != GPT_BF16) ||
+      T <= 0 || H <= 0 || H % kv->kv_heads || kv->batch == 0)
+    return 0;
+  return gpt::paged::make_plan(T, H, kv).bytes;
+}
+
+int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int64_t T,
+                                int64_t H, const gpt_paged_kv* kv, float scale, void* workspace, int64_t workspace_bytes,
+                                int dtype, void* stream) {
+  const char* what = "gpt_attention_shared_prefix";
+  GPT_CHECK_DTYPE(dtype);
+  int s = gpt::paged::check_kv(kv, what);
+  if (s) return s;
+  GPT_CHECK_SHAPE(T >= 0 && H > 0 && H % kv->kv_heads == 0, "%s: H=%lld must be a multiple of kv_heads=%lld, T=%lld", what,
+                  (long long)H, (long long)kv->kv_heads, (long long)T);
+  GPT_CHECK_SHAPE(T < (1LL << 30) && H < (1 << 20) && (kv->batch == 0 || T * H <= (1LL << 30) / kv->batch),
+                  "%s: more than 2^30 rows", what);
+  GPT_CHECK_ARG(scale > 0.f && isfinite(scale), "%s: scale must be positive and finite", what);
+  if (kv->batch == 0 || T == 0) return GPT_OK;
+  s = gpt::paged::check_kv_pointers(kv, what);
+  if (s) return s;
+  GPT_CHECK_ARG(q && out && q_strides && out_strides, "%s: null pointer", what);
+  const gpt::paged::Plan pl = gpt::paged::make_plan(T, H, kv);
+  GPT_CHECK_ARG(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes),
+                "%s: workspace of %lld bytes required", what, (long long)pl.bytes);
+  GPT_CHECK_ALIGN(pl.bytes == 0 || gpt::aligned(workspace, 16), "%s: workspace needs 16-byte alignment", what);
+  gpt::paged::Attn p = {};
+  p.q = q;
+  p.out = out;
+  p.q_b = q_strides[0];
+  p.q_h = q_strides[1];
+  p.q_t = q_strides[2];
+  p.o_b = out_strides[0];
+  p.o_h = out_strides[1];
+  p.o_t = out_strides[2];
+  p.k = kv->k_pages;
+  p.v = kv->v_pages;
+  p.page_stride = kv->page_stride;
+  p.head_stride = kv->head_stride;
+  p.slot_stride = kv->slot_stride;
+  p.n_pages = (int)kv->n_pages;
+  p.page = (int)kv->page_size;
+  p.table = kv->page_table;
+  p.ld_table = kv->ld_page_table;
+  p.cap = (int)(kv->max_pages * kv->page_size);
+  p.seq_lens = kv->seq_lens;
+  p.per = (int)kv->batch;
+  if (kv->n_groups > 0) {
+    p.ptable = kv->prefix_table;
+    p.ld_ptable = kv->ld_prefix_table;
+    p.pcap = (int)(kv->max_prefix_pages * kv->page_size);
+    p.plens = kv->prefix_lens;
+    p.per = (int)(kv->batch / kv->n_groups);
+  }
+  p.B = (int)kv->batch;
+  p.T = (int)T;
+  p.H = (int)H;
+  p.K = (int)kv->kv_heads;
+  p.share = (int)(H / kv->kv_heads);
+  p.D = (int)kv->head_dim;
+  p.scale_log2 = scale * gpt::paged::kLog2e;
+  const int64_t slots = pl.n_pre + (pl.n_own > 1 ? pl.n_own : 0);
+  p.ml = (float2*)workspace;
+  p.acc = (float*)workspace + 2 * slots * kv->batch * T * H;
+  cudaStream_t st = (cudaStream_t)stream;
+  return dtype == GPT_BF16 ? gpt::paged::run<__nv_bfloat16>(p, pl, st) : gpt::paged::run<float>(p, pl, st);
+}
+
+}  // extern "C"

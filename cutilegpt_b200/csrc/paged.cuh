@@ -1,0 +1,98 @@
+// The paged key/value cache as its kernels see it: where positions, rows and
+// partial results are, shared by paged_append.cu, paged_simt.cu and paged.cu.
+#pragma once
+
+#include "common.cuh"
+
+namespace gpt {
+namespace paged {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What a launch of an attention kernel looks at.
+//   kPrefix  the rows of all sequences of a group against the group's prefix
+//   kOwn     the rows of one sequence against its own positions
+//   kAll     the rows of one sequence against its prefix and then its own
+// The rows of a sequence and key head are (t, head of the group): r = t * share + h;
+// those of a group follow each other sequence by sequence.
+enum Phase { kPrefix = 0, kOwn = 1, kAll = 2 };
+
+struct Attn {
+  const void* q;
+  void* out;
+  int64_t q_b, q_h, q_t, o_b, o_h, o_t;   // element strides
+  const void* k;
+  const void* v;
+  int64_t page_stride, head_stride, slot_stride;
+  int n_pages, page;
+  const int32_t* table;
+  int64_t ld_table;
+  int cap;                  // own positions a table row can list
+  const int32_t* seq_lens;
+  const int32_t* ptable;
+  int64_t ld_ptable;
+  int pcap;
+  const int32_t* plens;
+  int B, T, H, K, share;    // share = H / K
+  int per;                  // sequences of a group (B without groups)
+  int D;
+  float scale_log2;
+  // Partial results, slot by slot: acc [slot][row][D] (sum of 2^(s - m) v), ml [slot][row] (m, sum of
+  // 2^(s - m)), row = (b * T + t) * H + h. Prefix parts are slots [0, n_pre), own parts n_pre ...
+  float* acc;
+  float2* ml;
+  int n_pre, n_own;
+};
+
+__device__ __forceinline__ int64_t row_id(const Attn& p, int b, int t, int h) {
+  return ((int64_t)b * p.T + t) * p.H + h;
+}
+
+// A length from device memory, clamped to what its table row can list.
+__device__ __forceinline__ int clamped_len(const int32_t* lens, int i, int cap) {
+  const int n = lens[i];
+  if (n < 0 || n > cap) {
+    record_device_error(GPT_DEVERR_INDEX);
+    return n < 0 ? 0 : cap;
+  }
+  return n;
+}
+__device__ __forceinline__ int own_len(const Attn& p, int b) { return clamped_len(p.seq_lens, b, p.cap); }
+__device__ __forceinline__ int prefix_len(const Attn& p, int g) {
+  return p.plens ? clamped_len(p.plens, g, p.pcap) : 0;
+}
+
+// Page id of a table entry, -1 (and the device error word) for one outside the pool.
+__device__ __forceinline__ int page_id(int id, int n_pages) {
+  if ((unsigned)id >= (unsigned)n_pages) {
+    record_device_error(GPT_DEVERR_INDEX);
+    return -1;
+  }
+  return id;
+}
+
+// The keys of a phase are positions 0 .. n_pre + n_own - 1: the prefix's first, then the own ones.
+struct Keys {
+  const int32_t* pre;
+  const int32_t* own;
+  int n_pre, n_own;
+  __device__ Keys(const Attn& p, int phase, int seq_or_group) {
+    const int b = phase == kPrefix ? seq_or_group * p.per : seq_or_group;
+    const int g = b / p.per;
+    n_pre = phase == kOwn ? 0 : prefix_len(p, g);
+    n_own = phase == kPrefix ? 0 : own_len(p, b);
+    pre = p.ptable + (int64_t)g * p.ld_ptable;
+    own = p.table + (int64_t)b * p.ld_table;
+  }
+  __device__ int n() const { return n_pre + n_own; }
+  // element offset of position j's row of head `kh`, -1 for a page outside the pool
+  __device__ int64_t offset(const Attn& p, int j, int kh) const {
+    const bool own_part = j >= n_pre;
+    const int i = own_part ? j - n_pre : j;
+    const int id = page_id((own_part ? own : pre)[i / p.page], p.n_pages);
+    return id < 0 ? -1 : id * p.page_stride + kh * p.head_stride + (int64_t)(i % p.page) * p.slot_stride;
+  }
+};
+
+}  // namespace paged
+}  // namespace gpt

@@ -5,6 +5,7 @@ from .linear import cutile_linear, cutile_linear_bias
 from .layernorm import cutile_layer_norm
 from .attention import cutile_causal_attention, cutile_mha_forward
 from .fused_mlp import cutile_fused_mlp
+from .paged import PagedKV, cutile_paged_kv_append, cutile_shared_prefix_attention
 
 __all__ = [
     'cutile_gelu',
@@ -14,4 +15,7 @@ __all__ = [
     'cutile_layer_norm',
     'cutile_causal_attention',
     'cutile_fused_mlp',
+    'PagedKV',
+    'cutile_paged_kv_append',
+    'cutile_shared_prefix_attention',
 ]

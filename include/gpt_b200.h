@@ -278,6 +278,81 @@ GPT_API int gpt_sample(const void* logits, int64_t ld, int64_t B, int64_t V,
                const int64_t* step_dev, int64_t step0, int64_t* out, int dtype,
                void* stream);
 
+/* ---- paged key/value cache (no reference counterpart) ------------------
+ * Keys and values live in pages of page_size positions: element (page, head,
+ * slot, d) of k_pages / v_pages is at page*page_stride + head*head_stride +
+ * slot*slot_stride + d (element strides, the same for both; d contiguous).
+ * The own positions of sequence b < batch are listed by row b of page_table
+ * [batch][max_pages] (row stride ld_page_table): position i is slot
+ * i % page_size of page page_table[b][i / page_size]. seq_lens[b] counts
+ * them, the new tokens of a call included; 0 is an idle slot of the batch.
+ * With n_groups > 0, sequence b also sees the positions that row
+ * b / (batch / n_groups) of prefix_table [n_groups][max_prefix_pages] lists,
+ * prefix_lens[group] of them, before its own (n_groups divides batch).
+ * Tables and lengths are int32 in device memory, so that a captured graph
+ * follows them. Table entries behind a length are not read, cache slots
+ * behind it may hold anything. A page id outside [0, n_pages), a negative
+ * length or one past the table's capacity is reported by gpt_device_error();
+ * such a page reads as zeros and is not written, such a length is clamped. */
+typedef struct gpt_paged_kv {
+  void* k_pages;
+  void* v_pages;
+  int64_t n_pages;
+  int64_t page_size;
+  int64_t kv_heads;
+  int64_t head_dim;
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t slot_stride;
+  const int32_t* page_table;
+  int64_t ld_page_table;
+  int64_t max_pages;
+  const int32_t* seq_lens;
+  int64_t batch;
+  const int32_t* prefix_table;
+  int64_t ld_prefix_table;
+  int64_t max_prefix_pages;
+  const int32_t* prefix_lens;
+  int64_t n_groups;
+} gpt_paged_kv;
+
+/* T new tokens of each sequence into the cache, their rotation on the way.
+ * Element (b, h, t, d) of q / q_out (H heads), k and v (kv_heads heads) is at
+ * b*s[0] + h*s[1] + t*s[2] + d. Token t of sequence b has own position
+ * i = seq_lens[b] - T + t; tokens with i < 0 are padding and are skipped
+ * (their q_out rows are zeros). With rot > 0 the first rot values of every
+ * query and key head are turned by position n = (prefix length) + i:
+ * pair j, (x[j], x[j + rot/2]) or with interleaved != 0 (x[2j], x[2j+1]),
+ * becomes (x0*c - x1*s, x0*s + x1*c), c = cos_sin[n][j], s =
+ * cos_sin[n][rot/2 + j] (fp32 [n_pos][rot]), in fp32, rounded once. A position
+ * at or past n_pos is reported by gpt_device_error() and gives zeros. q_out
+ * may alias q (same strides); without rotation q and q_out are not touched
+ * and may be NULL. */
+GPT_API int gpt_paged_kv_append(const void* q, const int64_t* q_strides,
+               const void* k, const int64_t* k_strides, const void* v,
+               const int64_t* v_strides, void* q_out,
+               const int64_t* q_out_strides, int64_t T, int64_t H,
+               const gpt_paged_kv* kv, const float* cos_sin, int64_t n_pos,
+               int64_t rot, int interleaved, int dtype, void* stream);
+
+/* Bytes of workspace gpt_attention_shared_prefix needs for these sizes (a
+ * function of the sizes in *kv, not of the lengths in device memory). */
+GPT_API int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H,
+               const gpt_paged_kv* kv, int dtype);
+
+/* Attention of the T newest tokens of each sequence over the paged cache:
+ * out[b, h, t] = softmax(scale * q . K) V over the prefix of b's group and its
+ * own positions 0 .. seq_lens[b] - T + t; head h reads key head
+ * h / (H / kv_heads). Rows of padding tokens (seq_lens[b] - T + t < 0) are
+ * zeros. What the sequences of a group share is read once for all of them;
+ * parts of the keys are computed apart and joined through `workspace`
+ * (gpt_attention_shared_prefix_workspace_size bytes, 16-byte aligned; NULL
+ * when that is 0). scale must be positive and finite. Strides as above. */
+GPT_API int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides,
+               void* out, const int64_t* out_strides, int64_t T, int64_t H,
+               const gpt_paged_kv* kv, float scale, void* workspace,
+               int64_t workspace_bytes, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
