@@ -32,12 +32,16 @@ import torch
 from .. import _lib as L
 from ..kernels import ops
 from ..kernels._common import as_cuda
+from ..kernels.paged import PagedKV
 from .config import GPTConfig
 from .init import init_state, weight_names
 
 # Greedy decode steps captured into one CUDA graph (the remainder of a
 # generate call replays the one-step graph).
 _GRAPH_STEPS = 8
+
+# Positions of a page of generate_samples' cache.
+_PAGE = 64
 
 
 class _Workspace:
@@ -59,11 +63,13 @@ class _Workspace:
 class _DecodeState:
     """Buffers of the KV-cache generation loop for one (B, Tmax)."""
 
-    def __init__(self, cfg: GPTConfig, B: int, Tmax: int, dtype, device, fold: bool = True):
+    def __init__(self, cfg: GPTConfig, B: int, Tmax: int, dtype, device, fold: bool = True, paged: bool = False):
         C, H = cfg.n_embd, cfg.n_head
         D = C // H
         self.B, self.Tmax = B, Tmax
-        self.cache = torch.empty((cfg.n_layer, 2, B, H, Tmax, D), dtype=dtype, device=device)
+        self.kv: Optional[list[PagedKV]] = None      # per layer, for a paged cache (_SampleState)
+        self.cache = (None if paged else
+                      torch.empty((cfg.n_layer, 2, B, H, Tmax, D), dtype=dtype, device=device))
         self.x = torch.empty((B, C), dtype=dtype, device=device)
         self.h = torch.empty((B, C), dtype=dtype, device=device)
         self.qkv = torch.empty((B, 3 * C), dtype=dtype, device=device)
@@ -73,7 +79,7 @@ class _DecodeState:
         self.tok = torch.empty((B,), dtype=torch.int64, device=device)
         self.pos = torch.zeros((1,), dtype=torch.int64, device=device)
         self.seq = torch.empty((B, Tmax), dtype=torch.int64, device=device)
-        nbytes = ops.decode_workspace_bytes(B, H, D, Tmax)
+        nbytes = 0 if paged else ops.decode_workspace_bytes(B, H, D, Tmax)
         self.dec_ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=device)
         self.graph: Optional[torch.cuda.CUDAGraph] = None          # greedy step
         self.graph_multi: Optional[torch.cuda.CUDAGraph] = None    # _GRAPH_STEPS greedy steps
@@ -87,6 +93,28 @@ class _DecodeState:
             # exact fp64 row totals (sum, sum of squares) of the residual stream: slot 2i = rows entering
             # block i, 2i+1 = after its attention, 2L = entering ln_f; slots >= 1 are accumulated into
             self.sums = torch.zeros((2 * cfg.n_layer + 1, B, 2), dtype=torch.float64, device=device)
+
+
+class _SampleState(_DecodeState):
+    """Buffers of generate_samples: `n` samples of each of `prompts` prompts over a paged cache whose
+    prompt pages all samples of a prompt share."""
+
+    def __init__(self, cfg: GPTConfig, prompts: int, n: int, T0: int, Tmax: int, dtype, device, fold: bool = True):
+        B, H = prompts * n, cfg.n_head
+        D, page = cfg.n_embd // H, _PAGE
+        super().__init__(cfg, B, Tmax, dtype, device, fold, paged=True)
+        n_pre, n_own = -(-T0 // page), -(-(Tmax - T0) // page)
+        pages = torch.empty((cfg.n_layer, 2, prompts * n_pre + B * n_own, H, page, D), dtype=dtype, device=device)
+        ids = torch.arange(pages.shape[2], dtype=torch.int32, device=device)
+        prefix = ids[:prompts * n_pre].view(prompts, n_pre)
+        own = ids[prompts * n_pre:].view(B, n_own)
+        lens = torch.full((prompts,), T0, dtype=torch.int32, device=device)
+        self.own_lens = torch.zeros((B,), dtype=torch.int32, device=device)
+        # per layer: the prompts as sequences of their own (prefill), and the samples behind them
+        self.prompt_kv = [PagedKV(p[0], p[1], prefix, lens) for p in pages]
+        self.kv = [PagedKV(p[0], p[1], own, self.own_lens, prefix, lens) for p in pages]
+        self.dec_ws = torch.empty((max(self.kv[0].workspace_bytes(H, 1) if self.kv else 0, 16),), dtype=torch.uint8,
+                                  device=device)
 
 
 class CutileGPT:
@@ -107,6 +135,7 @@ class CutileGPT:
         self.weight_transposes: Dict[str, torch.Tensor] = {}
         self._ws: Dict[Tuple[int, int], _Workspace] = {}
         self._dec: Dict[Tuple[int, int], _DecodeState] = {}
+        self._samples: Dict[Tuple[int, int, int, int], _SampleState] = {}
         # Optional object with start(flops) / stop() around every GEMM launch.
         self.kernel_timer = None
         # Folded decode step (default for bf16, up to 128 sequences; set False for the per-op step):
@@ -152,6 +181,7 @@ class CutileGPT:
             device=self.device, dtype=self.dtype).contiguous()
         self.weights = conv
         self._dec.clear()
+        self._samples.clear()
         self._folded = None
 
     def _check_shapes(self, state):
@@ -216,8 +246,18 @@ class CutileGPT:
             self._fold_weights()
         return ws
 
-    def _blocks(self, idx: torch.Tensor, ws: _Workspace, cache: Optional[torch.Tensor] = None) -> None:
-        """Embedding and all transformer blocks; appends K/V to `cache`. Result: ws.h = ln_f(x), or,
+    @staticmethod
+    def _store_kv(ws: _Workspace, cache, i: int, B: int, T: int) -> None:
+        """K/V of layer i's QKV rows into `cache`: a [n_layer, 2, B, H, Tmax, D] tensor, or a PagedKV per layer."""
+        if isinstance(cache, torch.Tensor):
+            ops.kv_append(ws.qkv.view(B, T, -1), cache[i, 0], cache[i, 1], pos0=0)
+        else:
+            kv = cache[i]
+            q4 = ws.qkv.view(B, T, 3, kv.n_kv_head, kv.head_dim)
+            ops.paged_kv_append(None, q4[:, :, 1].transpose(1, 2), q4[:, :, 2].transpose(1, 2), None, kv)
+
+    def _blocks(self, idx: torch.Tensor, ws: _Workspace, cache=None) -> None:
+        """Embedding and all transformer blocks; appends K/V to `cache` (see _store_kv). Result: ws.h = ln_f(x), or,
         with the LayerNorm fold (ws.fold), the residual stream ws.x and its row statistics ws.last_stats
         (ln_f is then applied by the lm_head GEMM, see _lm_head)."""
         cfg = self.config
@@ -241,7 +281,7 @@ class CutileGPT:
                 wf, u, v_ = F[p + 'attn']
                 self._gemm_fused(ws.x, wf, ws.qkv, epilogue=L.EPI_BIAS, ln=(cur, eps, u, v_))
                 if cache is not None:
-                    ops.kv_append(ws.qkv.view(B, T, 3 * C), cache[i, 0], cache[i, 1], pos0=0)
+                    self._store_kv(ws, cache, i, B, T)
                 ops.attention_prefill(q, k, v, att4, scale)
                 self._gemm_fused(ws.att, self._w(p + 'attn.c_proj.weight'), ws.x,
                                  bias=self._w(p + 'attn.c_proj.bias'), resid=ws.x, row_stats=ws.stats[1])
@@ -257,7 +297,7 @@ class CutileGPT:
             ops.layernorm(ws.x, self._w(p + 'ln_1.weight'), self._w(p + 'ln_1.bias'), ws.h)
             self._gemm(ws.h, self._w(p + 'attn.c_attn.weight'), ws.qkv, bias=self._w(p + 'attn.c_attn.bias'))
             if cache is not None:
-                ops.kv_append(ws.qkv.view(B, T, 3 * C), cache[i, 0], cache[i, 1], pos0=0)
+                self._store_kv(ws, cache, i, B, T)
             ops.attention_prefill(q, k, v, att4, scale)
             self._gemm(ws.att, self._w(p + 'attn.c_proj.weight'), ws.x, bias=self._w(p + 'attn.c_proj.bias'),
                      resid=ws.x)
@@ -298,8 +338,7 @@ class CutileGPT:
         else:
             self._gemm(ws.h, self._w('lm_head.weight'), out)
 
-    def forward_last(self, idx, out: Optional[torch.Tensor] = None,
-                     cache: Optional[torch.Tensor] = None) -> torch.Tensor:
+    def forward_last(self, idx, out: Optional[torch.Tensor] = None, cache=None) -> torch.Tensor:
         """Logits of the last position only, (batch, vocab): the prefill step of generation."""
         idx = self._prep_idx(idx)
         B, T = idx.shape
@@ -364,9 +403,12 @@ class CutileGPT:
                 p = f'h.{i}.'
                 wf, u, v = F[p + 'attn']
                 ops.gemm_fused(st.x, wf, st.qkv, epilogue=L.EPI_BIAS, ln=(st.sums[2 * i], eps, u, v),
-                               kv=(st.cache[i, 0], st.cache[i, 1], st.pos, 0))
-                ops.attention_decode(q, st.cache[i, 0], st.cache[i, 1], st.att, 1, st.dec_ws, scale,
-                                     len_dev=st.pos)
+                               kv=None if st.kv else (st.cache[i, 0], st.cache[i, 1], st.pos, 0))
+                if st.kv:
+                    self._paged_attention(st, i, scale)
+                else:
+                    ops.attention_decode(q, st.cache[i, 0], st.cache[i, 1], st.att, 1, st.dec_ws, scale,
+                                         len_dev=st.pos)
                 ops.gemm_fused(st.att, self._w(p + 'attn.c_proj.weight'), st.x, bias=self._w(p + 'attn.c_proj.bias'),
                                resid=st.x, row_stats=st.sums[2 * i + 1])
                 wf, u, v = F[p + 'fc']
@@ -380,9 +422,12 @@ class CutileGPT:
             p = f'h.{i}.'
             ops.layernorm(st.x, self._w(p + 'ln_1.weight'), self._w(p + 'ln_1.bias'), st.h)
             self._gemm(st.h, self._w(p + 'attn.c_attn.weight'), st.qkv, bias=self._w(p + 'attn.c_attn.bias'))
-            ops.kv_append(st.qkv.view(B, 1, 3 * C), st.cache[i, 0], st.cache[i, 1], pos0=0, pos_dev=st.pos)
-            ops.attention_decode(q, st.cache[i, 0], st.cache[i, 1], st.att, 1, st.dec_ws, scale,
-                                 len_dev=st.pos)
+            if st.kv:
+                self._paged_attention(st, i, scale)
+            else:
+                ops.kv_append(st.qkv.view(B, 1, 3 * C), st.cache[i, 0], st.cache[i, 1], pos0=0, pos_dev=st.pos)
+                ops.attention_decode(q, st.cache[i, 0], st.cache[i, 1], st.att, 1, st.dec_ws, scale,
+                                     len_dev=st.pos)
             self._gemm(st.att, self._w(p + 'attn.c_proj.weight'), st.x, bias=self._w(p + 'attn.c_proj.bias'),
                      resid=st.x)
             ops.layernorm(st.x, self._w(p + 'ln_2.weight'), self._w(p + 'ln_2.bias'), st.h)
@@ -393,16 +438,31 @@ class CutileGPT:
         ops.layernorm(st.x, self._w('ln_f.weight'), self._w('ln_f.bias'), st.h)
         self._gemm(st.h, self._w('lm_head.weight'), st.logits)
 
+    @staticmethod
+    def _paged_attention(st: _DecodeState, i: int, scale: float) -> None:
+        """Layer i's new keys and values into the paged cache, attention over it into st.att."""
+        kv = st.kv[i]
+        q, k, v = st.qkv.view(st.B, 1, 3, kv.n_kv_head, kv.head_dim).permute(2, 0, 3, 1, 4)   # [B, H, 1, D] views
+        ops.paged_kv_append(None, k, v, None, kv)
+        ops.shared_prefix_attention(q, kv, st.att.view(st.B, 1, kv.n_kv_head, kv.head_dim).transpose(1, 2), scale,
+                                    st.dec_ws)
+
     def _greedy_step(self, st: _DecodeState, seq: torch.Tensor) -> None:
         self._decode_step(st)
         ops.argmax(st.logits, st.tok)
+        self._advance(st, seq)
+
+    @staticmethod
+    def _advance(st: _DecodeState, seq: torch.Tensor) -> None:
         ops.decode_advance(st.tok, st.pos, seq)
+        if st.kv:
+            st.own_lens.add_(1)
 
     def _sample_step(self, st: _DecodeState, seq: torch.Tensor, temperature: float, top_k: Optional[int]) -> None:
         """Decode step + the sampling kernel; the draw is keyed by (seed, row, position of the token)."""
         self._decode_step(st)
         ops.sample(st.logits, st.tok, temperature, top_k, st.seed, st.pos)
-        ops.decode_advance(st.tok, st.pos, seq)
+        self._advance(st, seq)
 
     @staticmethod
     def _new_seed(generator: Optional[torch.Generator]) -> torch.Tensor:
@@ -450,8 +510,63 @@ class CutileGPT:
             ops.sample(st.logits, st.tok, temperature, top_k, st.seed, None, step0=T0 - 1)
         seq[:, T0] = st.tok
         st.pos.fill_(T0)
-        steps = max_new_tokens - 1
-        if not greedy:
+        self._decode_loop(st, max_new_tokens - 1, temperature, top_k, use_cuda_graph)
+        return seq.clone()
+
+    @torch.no_grad()
+    def generate_samples(self, idx, num_samples: int, max_new_tokens: int, temperature: float = 1.0,
+                         top_k: Optional[int] = None, use_cuda_graph: bool = True,
+                         generator: Optional[torch.Generator] = None) -> torch.Tensor:
+        """`num_samples` continuations of each prompt; (batch, num_samples, seq_len + max_new_tokens) int64.
+
+        A prompt is prefilled once and its keys and values are kept once, in pages that all its samples
+        share; each sample's own positions have pages of their own. Sample j of prompt i draws as row
+        i * num_samples + j of a batch does. Past block_size the windowed generation of `generate` runs
+        on the repeated prompts.
+        """
+        idx = self._prep_idx(idx)
+        P, T0 = idx.shape
+        if num_samples < 1:
+            raise ValueError(f"generate_samples: num_samples must be at least 1, got {num_samples}")
+        if max_new_tokens > 0 and top_k != 1 and temperature <= 0:
+            raise ValueError("temperature must be > 0")
+        total = T0 + max(0, max_new_tokens)
+        rows = idx.repeat_interleave(num_samples, dim=0)
+        if max_new_tokens <= 0 or total > self.config.block_size or rows.numel() == 0:
+            return self.generate(rows, max_new_tokens, temperature, top_k,
+                                 generator=generator).view(P, num_samples, total)
+        st = self._sample_state(P, num_samples, T0, total)
+        st.seq[:, :T0] = rows
+        first = self.forward_last(idx, cache=st.prompt_kv)
+        st.logits.view(P, num_samples, -1).copy_(first[:, None])
+        if top_k == 1:
+            ops.argmax(st.logits, st.tok)
+        else:
+            st.seed.copy_(self._new_seed(generator))
+            ops.sample(st.logits, st.tok, temperature, top_k, st.seed, None, step0=T0 - 1)
+        st.seq[:, T0] = st.tok
+        st.pos.fill_(T0)
+        st.own_lens.fill_(1)      # the decode step at hand appends own position 0
+        self._decode_loop(st, max_new_tokens - 1, temperature, top_k, use_cuda_graph)
+        return st.seq.clone().view(P, num_samples, total)
+
+    def _sample_state(self, P: int, n: int, T0: int, Tmax: int) -> _SampleState:
+        key = (P, n, T0, Tmax)
+        st = self._samples.get(key)
+        if st is None:
+            if len(self._samples) >= 2:
+                self._samples.pop(next(iter(self._samples)))
+            st = _SampleState(self.config, P, n, T0, Tmax, self.dtype, self.device, fold=self.fold_decode)
+            self._samples[key] = st
+        if st.fold:
+            self._fold_weights()   # eager, outside any graph capture
+        return st
+
+    def _decode_loop(self, st: _DecodeState, steps: int, temperature: float, top_k: Optional[int],
+                     use_cuda_graph: bool) -> None:
+        """`steps` decode steps from st.tok at device position *st.pos, tokens into st.seq."""
+        seq = st.seq
+        if top_k != 1:
             key = (float(temperature), 0 if top_k is None else int(top_k))
             g = st.sample_graphs.get(key)
             if not use_cuda_graph or (g is None and steps < 2):
@@ -486,7 +601,6 @@ class CutileGPT:
                 st.graph_multi.replay()
             for _ in range(steps % _GRAPH_STEPS):
                 st.graph.replay()
-        return seq.clone()
 
     def _capture_fn(self, fn) -> torch.cuda.CUDAGraph:
         g = torch.cuda.CUDAGraph()
