@@ -79,6 +79,12 @@ static int run(Attn& p, const Plan& pl, cudaStream_t st) {
   p.n_pre = pl.n_pre;
   p.n_own = pl.n_own > 1 ? pl.n_own : 0;
   int s = GPT_OK;
+  if (sizeof(T) == 2 && rows_eligible(p)) {
+    if (pl.shared) s = launch_rows(p, kPrefix, pl.n_pre, 0, 0, 0, st);
+    if (!s) s = launch_rows(p, pl.shared ? kOwn : kAll, pl.n_own, pl.n_pre, pl.n_own == 1, pl.shared, st);
+    if (!s && pl.n_own > 1) s = launch_join<T>(p, st);
+    return s;
+  }
   if (pl.shared) s = launch_simt<T>(p, kPrefix, pl.n_pre, 0, 0, st);
   if (!s) s = launch_simt<T>(p, pl.shared ? kOwn : kAll, pl.n_own, pl.n_pre, pl.n_own == 1, st);
   if (!s && pl.n_own > 1) s = launch_join<T>(p, st);

@@ -1,0 +1,349 @@
+// Attention over the paged cache for few rows a key head (bf16): one decode
+// step, or the few tokens of a draft.
+//
+// Every key and value is read once and meets at most 16 rows, so the kernel is
+// bound by HBM: 4 D bytes a key against 64 D multiply-adds. A CTA takes 16 rows
+// of one key head (phases as in paged.cuh) and one of `splits` equal shares of
+// the phase's keys. Its four warps work alone until the end: warp w takes the
+// steps of KS keys w, w + 4, ... of the share, copies them by cp.async
+// (16 bytes a lane, addresses from the page table, zeros behind the length) into its
+// own ring of kRing steps, and keeps running maxima, sums and the 16 x D
+// accumulator in registers: S = Q Kᵀ and O += P V are m16n8k16 tensor-core
+// products (16 rows cannot fill the 128 rows of a tcgen05 tile; those run in
+// paged_tc.cu). No barrier stands between a warp's loads and its products, so a
+// CTA keeps 4 x (kRing - 1) steps of 8 KB in flight, two CTAs of an SM 128 KB.
+// P is rounded to bf16 for the product with V (as the V it meets); its sum is
+// taken before the rounding, in fp32.
+#include "paged.cuh"
+
+namespace gpt {
+namespace paged {
+
+constexpr int kRowTile = 16;
+constexpr int kRowWarps = 4;
+constexpr int kRing = 3;
+
+// Keys of a warp's step: 8 KB of keys and values, at most 64 keys.
+constexpr int step_keys(int dp) { return 2048 / dp < 64 ? 2048 / dp : 64; }
+constexpr int rows_smem(int dp) {
+  const int ring = kRowWarps * kRing * step_keys(dp) * dp * 4, merge = kRowWarps * kRowTile * (dp + 4) * 4;
+  return ring > merge ? ring : merge;
+}
+
+// Byte offset of 16-byte chunk c of row r in a tile of rows of DP bf16, chunks permuted
+// inside a row so that eight consecutive rows of one chunk column hit eight bank groups.
+template <int DP>
+__device__ __forceinline__ uint32_t swz(int r, int c) {
+  constexpr int kChunks = DP / 8;
+  const int x = kChunks >= 8 ? (r & 7) : kChunks == 4 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+  return (uint32_t)(r * DP * 2 + ((c ^ x) << 4));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// One row's four columns joined with the partial slots first .. first + n - 1.
+__device__ __forceinline__ void join4(const Attn& p, int first, int n, int64_t row, int d, float& m, float& l, float4& acc) {
+  const int64_t rows = (int64_t)p.B * p.T * p.H;
+  const float2* ml = p.ml + first * rows + row;
+  float top = l == 0.f ? -INFINITY : m;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float2 o = ml[s * rows];
+    if (o.y != 0.f) top = fmaxf(top, o.x);
+  }
+  const float a = l == 0.f ? 0.f : exp2f(m - top);
+  m = top;
+  l *= a;
+  acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll 4
+  for (int s = 0; s < n; ++s) {
+    const float2 o = ml[s * rows];
+    if (o.y == 0.f) continue;   // no keys: its accumulator was not written
+    const float w = exp2f(o.x - top);
+    const float4 v = *reinterpret_cast<const float4*>(p.acc + ((int64_t)(first + s) * rows + row) * p.D + d);
+    l = fmaf(o.y, w, l);
+    acc.x = fmaf(v.x, w, acc.x);
+    acc.y = fmaf(v.y, w, acc.y);
+    acc.z = fmaf(v.z, w, acc.z);
+    acc.w = fmaf(v.w, w, acc.w);
+  }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Attn p, int phase, int splits, int blocks,
+                                                                       int slot0, int direct, int early) {
+  constexpr int KS = step_keys(DP), kChunks = DP / 8, kLoads = KS * kChunks / 32;
+  constexpr int kTile = KS * DP * 2;                  // bytes of a step's keys
+  extern __shared__ __align__(128) uint8_t rows_smem_dyn[];
+  // With `early` the launch before is this call's prefix launch, whose every CTA has waited for all
+  // that came before it: what is read and written here is then safe, but for the prefix's partial results.
+  if (!early) pdl_wait();
+  pdl_trigger();
+  int item = blockIdx.x;
+  const int split = item % splits;
+  item /= splits;
+  const int block = item % blocks;
+  item /= blocks;
+  const int kh = item % p.K, who = item / p.K;
+  const int b0 = phase == kPrefix ? who * p.per : who;
+  const int rs = p.T * p.share;                       // rows of a sequence
+  const int rows = rs * (phase == kPrefix ? p.per : 1);
+  const int r0 = block * kRowTile;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Keys keys(p, phase, who);
+  const int n = keys.n();
+  const int chunk = ((n + splits - 1) / splits + KS - 1) / KS * KS;
+  const int j0 = min(n, split * chunk);
+  int j1 = min(n, j0 + chunk);
+
+  // Q in the A fragments: rows lane / 4 and lane / 4 + 8
+  uint32_t qf[DP / 16][4];
+  int seen[2];        // keys below this one are the row's
+  int most = 0;       // largest of the tile's
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = r0 + lane / 4 + 8 * half;
+    const bool live = r < rows;
+    const int b = b0 + (live ? r / rs : 0), rr = live ? r % rs : 0, t = rr / p.share;
+    seen[half] = !live ? 0 : phase == kPrefix ? n : max(0, keys.n_pre + keys.n_own - p.T + t + 1);
+    if (live && phase != kPrefix && keys.n_own - p.T + t < 0) seen[half] = 0;   // padding sees nothing
+    most = max(most, seen[half]);
+    const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + b * p.q_b + (int64_t)(kh * p.share + rr % p.share) * p.q_h + t * p.q_t;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int d = k * 16 + c * 8 + (lane & 3) * 2;
+        qf[k][half + 2 * c] = live && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+      }
+  }
+  j1 = min(j1, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
+
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem_dyn) + warp * (kRing * 2 * kTile);
+  if (p.D < DP) {   // columns behind D stay zeros
+    for (int i = threadIdx.x; i < rows_smem(DP) / 16; i += blockDim.x) reinterpret_cast<uint4*>(rows_smem_dyn)[i] = uint4{};
+    __syncthreads();
+  }
+  const int steps = j1 > j0 + warp * KS ? (j1 - j0 - warp * KS + kRowWarps * KS - 1) / (kRowWarps * KS) : 0;
+  // lane i holds the offsets of keys i, i + 32, ... of a step, -1 where there is none
+  constexpr int kOffs = (KS + 31) / 32;
+  int64_t off[kOffs];
+  auto locate = [&](int s) {
+#pragma unroll
+    for (int i = 0; i < kOffs; ++i) {
+      const int in = lane + 32 * i, j = j0 + (s * kRowWarps + warp) * KS + in;
+      off[i] = in < KS && s < steps && j < j1 ? keys.offset(p, j, kh) : -1;
+    }
+  };
+  auto fetch = [&](int s) {
+    const uint32_t dst = ring + (uint32_t)(s % kRing) * (2 * kTile);
+    const int c = lane % kChunks;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int r = i * (32 / kChunks) + lane / kChunks;
+      const int64_t o = __shfl_sync(0xffffffffu, off[i * (32 / kChunks) / 32], r & 31);
+      if (c * 8 < p.D) {
+        const int64_t at = (o < 0 ? 0 : o) + c * 8;
+        cp_async16(dst + swz<DP>(r, c), (const __nv_bfloat16*)p.k + at, o >= 0);
+        cp_async16(dst + kTile + swz<DP>(r, c), (const __nv_bfloat16*)p.v + at, o >= 0);
+      }
+    }
+    cp_commit();
+  };
+
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DP / 8][4];
+#pragma unroll
+  for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+  for (int s = 0; s < kRing - 1; ++s) {
+    locate(s);
+    fetch(s);
+  }
+  locate(kRing - 1);
+  for (int s = 0; s < steps; ++s) {
+    cp_wait<kRing - 2>();
+    __syncwarp();
+    fetch(s + kRing - 1);      // into the slot of step s - 1, which every lane has left
+    locate(s + kRing);         // the table read is on its way while this step computes
+    const uint32_t sk = ring + (uint32_t)(s % kRing) * (2 * kTile), sv = sk + kTile;
+    const int j = j0 + (s * kRowWarps + warp) * KS;
+    float sc[KS / 8][4];
+#pragma unroll
+    for (int i = 0; i < KS / 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sc[i][k] = 0.f;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < KS / 16; ++i) {
+        uint32_t kb[4];
+        ldsm4(sk + swz<DP>(i * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + ((lane >> 3) & 1)), kb);
+        mma16816(sc[2 * i], qf[k], kb[0], kb[1]);
+        mma16816(sc[2 * i + 1], qf[k], kb[2], kb[3]);
+      }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < KS / 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int at = j + i * 8 + (lane & 3) * 2 + (k & 1);
+        sc[i][k] = at < min(j1, seen[k >> 1]) ? sc[i][k] * p.scale_log2 : -INFINITY;
+        mx[k >> 1] = fmaxf(mx[k >> 1], sc[i][k]);
+      }
+    float base[2], a[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      const float mn = fmaxf(m[h], mx[h]);
+      base[h] = mn == -INFINITY ? 0.f : mn;      // a row without keys so far: every 2^(s - base) is 0
+      a[h] = exp2f(m[h] - base[h]);
+      m[h] = mn;
+      l[h] *= a[h];
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] *= a[k >> 1];
+#pragma unroll
+    for (int i = 0; i < KS / 16; ++i) {
+      uint32_t pf[4];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e0 = exp2f(sc[2 * i + c][2 * h] - base[h]), e1 = exp2f(sc[2 * i + c][2 * h + 1] - base[h]);
+          l[h] += e0 + e1;
+          pf[h + 2 * c] = tc::pack2_bf16(e0, e1);
+        }
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        uint32_t vb[4];
+        ldsm4_t(sv + swz<DP>(i * 16 + (lane & 15), d * 2 + (lane >> 4)), vb);
+        mma16816(o[2 * d], pf, vb[0], vb[1]);
+        mma16816(o[2 * d + 1], pf, vb[2], vb[3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+  }
+
+  // the warps' results joined through shared memory, where the rings were
+  cp_wait<0>();
+  __syncthreads();
+  float* sm_o = reinterpret_cast<float*>(rows_smem_dyn);            // [warp][16][DP]
+  float2* sm_ml = reinterpret_cast<float2*>(sm_o + kRowWarps * kRowTile * DP);   // [warp][16]
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = lane / 4 + 8 * h;
+    if ((lane & 3) == 0) sm_ml[warp * kRowTile + r] = make_float2(m[h], l[h]);
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i)
+      *reinterpret_cast<float2*>(sm_o + (warp * kRowTile + r) * DP + i * 8 + (lane & 3) * 2) =
+          make_float2(o[i][2 * h], o[i][2 * h + 1]);
+  }
+  __syncthreads();
+  if (early) pdl_wait();   // the prefix launch's partial results; its end, for whatever comes after this launch
+  const int live = min(kRowTile, rows - r0), quads = p.D / 4;
+  for (int i = threadIdx.x; i < live * quads; i += blockDim.x) {
+    const int rl = i / quads, d = i % quads * 4, r = r0 + rl;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm_ml[w * kRowTile + rl].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const float2 ml = sm_ml[w * kRowTile + rl];
+      const float c = ml.y == 0.f ? 0.f : exp2f(ml.x - top);
+      const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * kRowTile + rl) * DP + d);
+      sum = fmaf(ml.y, c, sum);
+      acc.x = fmaf(v.x, c, acc.x);
+      acc.y = fmaf(v.y, c, acc.y);
+      acc.z = fmaf(v.z, c, acc.z);
+      acc.w = fmaf(v.w, c, acc.w);
+    }
+    const int b = b0 + r / rs, t = r % rs / p.share, h = kh * p.share + r % rs % p.share;
+    const int64_t row = row_id(p, b, t, h);
+    if (direct) {
+      const bool padding = keys.n_own - p.T + t < 0;
+      if (!padding && p.n_pre > 0) join4(p, 0, p.n_pre, row, d, top, sum, acc);
+      const float inv = padding ? 0.f : 1.f / sum;
+      uint2 w;
+      w.x = padding ? 0u : tc::pack2_bf16(acc.x * inv, acc.y * inv);
+      w.y = padding ? 0u : tc::pack2_bf16(acc.z * inv, acc.w * inv);
+      *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d) = w;
+    } else {
+      const int64_t at = (int64_t)(slot0 + split) * p.B * p.T * p.H + row;
+      if (d == 0) p.ml[at] = make_float2(top, sum);
+      if (sum != 0.f) *reinterpret_cast<float4*>(p.acc + at * p.D + d) = acc;
+    }
+  }
+}
+
+// Whether the kernel serves the call: 16-byte rows of keys and values, 4-byte pairs of q, 8-byte quads of out.
+static bool rows_eligible(const Attn& p) {
+  if (p.D % 8 || p.D > 128 || !aligned(p.k, 16) || !aligned(p.v, 16) || !aligned(p.q, 4) || !aligned(p.out, 8)) return false;
+  return p.page_stride % 8 == 0 && p.head_stride % 8 == 0 && p.slot_stride % 8 == 0 && p.q_b % 2 == 0 && p.q_h % 2 == 0 &&
+         p.q_t % 2 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && p.o_t % 4 == 0;
+}
+
+template <int DP>
+static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+  static bool done[64] = {false};
+  static std::mutex mu;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> g(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem(DP));
+      if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      done[dev] = true;
+    }
+  }
+  const int64_t rows = (int64_t)p.T * p.share * (phase == kPrefix ? p.per : 1);
+  const int64_t blocks = (rows + kRowTile - 1) / kRowTile;
+  const int64_t grid = blocks * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
+  GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
+  launch_pdl(paged_rows_kernel<DP>, dim3((unsigned)grid), dim3(kRowWarps * 32), rows_smem(DP), st, p, phase, splits,
+             (int)blocks, slot0, direct, early);
+  return launch_status("paged_rows");
+}
+
+static int launch_rows(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+  if (p.D <= 16) return launch_rows_dp<16>(p, phase, splits, slot0, direct, early, st);
+  if (p.D <= 32) return launch_rows_dp<32>(p, phase, splits, slot0, direct, early, st);
+  if (p.D <= 64) return launch_rows_dp<64>(p, phase, splits, slot0, direct, early, st);
+  return launch_rows_dp<128>(p, phase, splits, slot0, direct, early, st);
+}
+
+}  // namespace paged
+}  // namespace gpt
