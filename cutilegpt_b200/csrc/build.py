@@ -18,7 +18,7 @@ LIB_PATH = os.path.join(LIB_DIR, "libgpt_b200.so")
 SOURCES = ["libgpt_b200.cu", "common.cuh", "capi.cu", "elementwise.cu", "gemm_tc.cu", "gemm_skinny.cu", "gemm_rows.cu",
            "gemm_simt.cu", "attention_tc.cu", "attention.cu", "decode.cu", "decode_noalloc.cu",
            "sampling.cu", "paged.cuh", "paged_append.cu", "paged_simt.cu",
-           "paged_rows.cu", "paged.cu"]
+           "paged_rows.cu", "paged_tc.cu", "paged.cu"]
 HEADER = os.path.join(os.path.dirname(PKG), "include", "gpt_b200.h")
 
 NVCC_FLAGS = [

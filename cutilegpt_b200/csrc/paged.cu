@@ -38,56 +38,96 @@ static int check_kv_pointers(const gpt_paged_kv* kv, const char* what) {
   return GPT_OK;
 }
 
+// The kernels of an attention call, in the order of preference for the calls that they can serve.
+enum Kernel { kSimt = 0, kRows = 1, kTc = 2 };
+
 // How an attention call runs.
 struct Plan {
-  int shared;          // the prefix apart from the own positions, once for a group
-  int n_pre, n_own;    // shares of the keys with partial results of their own; n_own = 1: the last launch writes out
-  int64_t bytes;       // workspace
+  int shared;              // the prefix apart from the own positions, once for a group
+  Kernel pre, own;         // kernels of the two launches (own: of the only one without `shared`)
+  int pre_splits, pre_two, own_splits, own_two;
+  int n_pre, n_own;        // slots of partial results; n_own = 0: the own launch writes out
+  int64_t acc_floats;      // of the workspace: the accumulators, then the rows' (m, l)
+  int64_t bytes;           // workspace
 };
 
-// Shares of `keys` keys for `items` CTAs of equal work: enough for two CTAs on every SM, at
-// least 128 keys in a share.
-static int shares(int64_t items, int64_t keys, int sms) {
-  const int64_t want = (2 * (int64_t)sms + items - 1) / (items > 0 ? items : 1);
-  const int64_t most = (keys + 127) / 128;
+// Rows of a sequence and key head up to which the few-row kernel takes them.
+constexpr int kFewRows = 16;
+// Rows from which a sequence reads its group's prefix by itself: it fills a 128-row tile alone.
+constexpr int kOwnTile = 128;
+
+// Equal shares of `keys` keys for `items` CTAs: enough for `per_sm` CTAs on every SM, at least `least` keys in a share.
+static int shares(int64_t items, int64_t keys, int sms, int per_sm, int64_t least) {
+  const int64_t want = (per_sm * (int64_t)sms + items - 1) / (items > 0 ? items : 1);
+  const int64_t most = (keys + least - 1) / least;
   const int64_t s = want < most ? want : most;
   return (int)(s < 1 ? 1 : s > 256 ? 256 : s);
 }
 
-static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv) {
+static void plan_launch(Kernel kernel, int64_t rows, int64_t items, int64_t keys, int sms, int* splits, int* two,
+                        int* slots) {
+  *two = kernel == kTc && rows > 128;
+  if (kernel == kTc) {
+    // one CTA on an SM: no more than fit at once, at least two tiles for a pipeline
+    items *= (rows + (*two ? 255 : 127)) / (*two ? 256 : 128);
+    const int64_t most = (keys + (*two ? 255 : 511)) / (*two ? 256 : 512), want = sms / (items > 0 ? items : 1);
+    *splits = (int)(want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most);
+    *slots = *two ? *splits : 2 * *splits;
+  } else {
+    *splits = shares(items * ((rows + 15) / 16), keys, sms, 2, 128);
+    *slots = *splits;
+  }
+}
+
+// The plan for the best kernel allowed.
+static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, Kernel best) {
   int sms = device_sm_count();
   if (sms <= 0) sms = 148;
   Plan pl = {};
   const int64_t groups = kv->n_groups, per = groups > 0 ? kv->batch / groups : kv->batch;
-  const int64_t share = H / kv->kv_heads, own_keys = kv->max_pages * kv->page_size;
+  const int64_t rows = T * (H / kv->kv_heads), own_keys = kv->max_pages * kv->page_size;
   const int64_t pre_keys = groups > 0 ? kv->max_prefix_pages * kv->page_size : 0;
-  pl.shared = groups > 0 && per > 1;
-  const int64_t own_blocks = (T * share + 15) / 16, pre_blocks = (per * T * share + 15) / 16;
-  if (pl.shared) {
-    pl.n_pre = shares(groups * kv->kv_heads * pre_blocks, pre_keys, sms);
-    pl.n_own = shares(kv->batch * kv->kv_heads * own_blocks, own_keys, sms);
-  } else {
-    pl.n_own = shares(kv->batch * kv->kv_heads * own_blocks, own_keys + pre_keys, sms);
-  }
-  const int64_t slots = pl.n_pre + (pl.n_own > 1 ? pl.n_own : 0);
-  pl.bytes = slots * kv->batch * T * H * (kv->head_dim + 2) * (int64_t)sizeof(float);
+  pl.shared = groups > 0 && per > 1 && (best != kTc || rows < kOwnTile);
+  pl.pre = best;
+  pl.own = best == kTc && rows <= kFewRows ? kRows : best;
+  if (pl.shared) plan_launch(pl.pre, rows * per, groups * kv->kv_heads, pre_keys, sms, &pl.pre_splits, &pl.pre_two, &pl.n_pre);
+  plan_launch(pl.own, rows, kv->batch * kv->kv_heads, own_keys + (pl.shared ? 0 : pre_keys), sms, &pl.own_splits, &pl.own_two,
+              &pl.n_own);
+  // one share: the kernel joins the prefix's slots itself and writes out (the tcgen05 kernel: where there are none)
+  if (pl.n_own == 1 && (pl.own != kTc || pl.n_pre == 0)) pl.n_own = 0;
+  const int64_t parts = (int64_t)(pl.n_pre + pl.n_own) * kv->batch * T * H;
+  pl.acc_floats = (parts * kv->head_dim + 3) / 4 * 4;
+  pl.bytes = (pl.acc_floats + 2 * parts) * (int64_t)sizeof(float);
   return pl;
+}
+
+template <typename T>
+static int launch(Kernel kernel, const Attn& p, int phase, int splits, int two, int slot0, int direct, int early,
+                  cudaStream_t st) {
+  if constexpr (sizeof(T) == 2) {
+    if (kernel == kTc) {
+      TcArgs a = {};
+      a.phase = phase;
+      a.splits = splits;
+      a.two = two;
+      a.slot0 = slot0;
+      a.direct = direct;
+      a.early = early;
+      return launch_tc(p, a, st);
+    }
+    if (kernel == kRows) return launch_rows(p, phase, splits, slot0, direct, early, st);
+  }
+  return launch_simt<T>(p, phase, splits, slot0, direct, st);
 }
 
 template <typename T>
 static int run(Attn& p, const Plan& pl, cudaStream_t st) {
   p.n_pre = pl.n_pre;
-  p.n_own = pl.n_own > 1 ? pl.n_own : 0;
+  p.n_own = pl.n_own;
   int s = GPT_OK;
-  if (sizeof(T) == 2 && rows_eligible(p)) {
-    if (pl.shared) s = launch_rows(p, kPrefix, pl.n_pre, 0, 0, 0, st);
-    if (!s) s = launch_rows(p, pl.shared ? kOwn : kAll, pl.n_own, pl.n_pre, pl.n_own == 1, pl.shared, st);
-    if (!s && pl.n_own > 1) s = launch_join<T>(p, st);
-    return s;
-  }
-  if (pl.shared) s = launch_simt<T>(p, kPrefix, pl.n_pre, 0, 0, st);
-  if (!s) s = launch_simt<T>(p, pl.shared ? kOwn : kAll, pl.n_own, pl.n_pre, pl.n_own == 1, st);
-  if (!s && pl.n_own > 1) s = launch_join<T>(p, st);
+  if (pl.shared) s = launch<T>(pl.pre, p, kPrefix, pl.pre_splits, pl.pre_two, 0, 0, 0, st);
+  if (!s) s = launch<T>(pl.own, p, pl.shared ? kOwn : kAll, pl.own_splits, pl.own_two, pl.n_pre, pl.n_own == 0, pl.shared, st);
+  if (!s && pl.n_own > 0) s = launch_join<T>(p, st);
   return s;
 }
 
@@ -173,7 +213,13 @@ int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H, const g
   if (gpt::paged::check_kv(kv, "gpt_attention_shared_prefix_workspace_size") || (dtype != GPT_F32 && dtype != GPT_BF16) ||
       T <= 0 || H <= 0 || H % kv->kv_heads || kv->batch == 0)
     return 0;
-  return gpt::paged::make_plan(T, H, kv).bytes;
+  // the largest over the kernels that the alignment of q and out may ask for
+  int64_t most = 0;
+  for (int k = gpt::paged::kSimt; k <= (dtype == GPT_BF16 ? gpt::paged::kTc : gpt::paged::kSimt); ++k) {
+    const int64_t n = gpt::paged::make_plan(T, H, kv, (gpt::paged::Kernel)k).bytes;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int64_t T,
@@ -192,10 +238,6 @@ int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* o
   s = gpt::paged::check_kv_pointers(kv, what);
   if (s) return s;
   GPT_CHECK_ARG(q && out && q_strides && out_strides, "%s: null pointer", what);
-  const gpt::paged::Plan pl = gpt::paged::make_plan(T, H, kv);
-  GPT_CHECK_ARG(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes),
-                "%s: workspace of %lld bytes required", what, (long long)pl.bytes);
-  GPT_CHECK_ALIGN(pl.bytes == 0 || gpt::aligned(workspace, 16), "%s: workspace needs 16-byte alignment", what);
   gpt::paged::Attn p = {};
   p.q = q;
   p.out = out;
@@ -231,9 +273,16 @@ int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* o
   p.share = (int)(H / kv->kv_heads);
   p.D = (int)kv->head_dim;
   p.scale_log2 = scale * gpt::paged::kLog2e;
-  const int64_t slots = pl.n_pre + (pl.n_own > 1 ? pl.n_own : 0);
-  p.ml = (float2*)workspace;
-  p.acc = (float*)workspace + 2 * slots * kv->batch * T * H;
+  const gpt::paged::Kernel best = dtype != GPT_BF16              ? gpt::paged::kSimt
+                                  : gpt::paged::tc_eligible(p)   ? gpt::paged::kTc
+                                  : gpt::paged::rows_eligible(p) ? gpt::paged::kRows
+                                                                 : gpt::paged::kSimt;
+  const gpt::paged::Plan pl = gpt::paged::make_plan(T, H, kv, best);
+  GPT_CHECK_ARG(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes),
+                "%s: workspace of %lld bytes required", what, (long long)pl.bytes);
+  GPT_CHECK_ALIGN(pl.bytes == 0 || gpt::aligned(workspace, 16), "%s: workspace needs 16-byte alignment", what);
+  p.acc = (float*)workspace;
+  p.ml = (float2*)((float*)workspace + pl.acc_floats);
   cudaStream_t st = (cudaStream_t)stream;
   return dtype == GPT_BF16 ? gpt::paged::run<__nv_bfloat16>(p, pl, st) : gpt::paged::run<float>(p, pl, st);
 }

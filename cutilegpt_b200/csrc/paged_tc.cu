@@ -1,0 +1,462 @@
+// Attention over the paged cache on the 5th-generation tensor cores (bf16,
+// head sizes 64 and 128): the rows of all sequences of a group against the
+// prefix that they share, and the many rows of long questions.
+//
+// A CTA takes 128 or 256 rows of one key head (phases and rows as in paged.cuh) and
+// one of `splits` equal shares of the phase's key tiles. A tile is up to 128 keys:
+// whole pages, each copied by one TMA box per 64 columns from {D, slot, head, page} maps (a page past the
+// pool is out of the map's bounds: zeros). Two pipelines of one softmax
+// warpgroup (one thread per row = TMEM lane) and one MMA-issuing lane work on
+//   two != 0: the same tiles, pipeline s on rows 128 s .. of the block, so that 256
+//             rows share one reading of the keys,
+//   two == 0: the same 128 rows, pipeline s on tiles s, s + 2, ... of the share, each with a
+//             partial result of its own,
+// so that one's products run while the other's softmax does. Per tile:
+//   S = Q Kᵀ      tcgen05.mma M=128 N=128 K=D -> TMEM
+//   softmax       the row's 128 scores are read into registers, masked (the row's keys end inside a
+//                 tile), P = 2^(scale S - m) to TMEM as bf16, the sum of P before its rounding in fp32
+//   O += P V      A = P from TMEM, B = V MN-major as its boxes arrive; only the 16-key steps
+//                 that hold keys are issued, and the last one's rows behind the keys are cleared
+//                 first: what the cache holds there must not meet P = 0
+// m moves only when a tile's maximum exceeds it by 2^8 (then O and the sum are
+// rescaled), so P stays below 2^8 and O / l is the same softmax. With D = 64 P has
+// TMEM columns of its own and the next S is computed under the softmax; with D = 128
+// P takes the place of S (256 columns a pipeline), and the next S follows the PV.
+// Keys and values have separate rings; every wait is bounded.
+#include "paged.cuh"
+
+namespace gpt {
+namespace paged {
+
+using attn_tc::ex2;
+using attn_tc::fadd2;
+using attn_tc::ffma2;
+using attn_tc::fmax3;
+using attn_tc::pack_f2;
+using attn_tc::pack_u2;
+using attn_tc::tc_mma_ts;
+using attn_tc::tmem_ld32_nw;
+using attn_tc::tmem_st16;
+using attn_tc::tmem_st32;
+using attn_tc::tmem_wait_ld;
+using attn_tc::tmem_wait_st;
+using attn_tc::tma_load_4d;
+using attn_tc::unpack_f2;
+using tc::desc_sw128;
+using tc::mbar_arrive;
+using tc::mbar_expect_tx;
+using tc::mbar_init;
+using tc::mbar_wait;
+using tc::smem_addr;
+using tc::tc_commit;
+using tc::tc_fence_after;
+using tc::tc_fence_before;
+using tc::tc_mma;
+using tc::tmem_ld32;
+
+constexpr int kTcThreads = 12 * 32;      // 2 x 4 softmax warps, 2 MMA warps, K and V copy warps
+constexpr int kPanel = 128 * 128;        // 128 rows of 64 bf16, 128-byte swizzled
+constexpr float kTcRescale = 8.f;        // log2 of the largest P before O is rescaled
+
+template <int D>
+struct Tc {
+  static constexpr int kPanels = D / 64;
+  static constexpr int kTile = kPanels * kPanel;         // a Q, K or V tile
+  static constexpr int kStages = D == 64 ? 5 : 2;        // of each ring: 160 or 128 KB in flight
+  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kStages * kTile + 512;
+  static constexpr bool kAlias = D == 128;               // P in the columns of S
+  static constexpr uint32_t kP = kAlias ? 0 : 128, kO = kAlias ? 128 : 192;
+};
+
+struct TcArgs {
+  int phase, splits, blocks, slot0, direct, early, two;
+  int tile;   // keys of a tile
+  int box;    // keys of a TMA box
+};
+
+template <int D>
+__global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ CUtensorMap tk,
+                                                                 const __grid_constant__ CUtensorMap tv, const Attn p,
+                                                                 const TcArgs a) {
+  using C = Tc<D>;
+  constexpr int ST = C::kStages;
+  extern __shared__ uint8_t tc_smem_dyn[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)tc_smem_dyn + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = base;                       // [2][kTile]
+  uint8_t* sK = sQ + 2 * C::kTile;          // [ST][kTile]
+  uint8_t* sV = sK + ST * C::kTile;         // [ST][kTile]
+  uint64_t* bars = (uint64_t*)(sV + ST * C::kTile);
+  uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST;
+  uint64_t* pipe_bars = bars + 4 * ST;      // per pipeline: q_full, s_full, s_free, p_full, o_full
+  uint32_t* tmem_slot = (uint32_t*)(pipe_bars + 10);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (!a.early) pdl_wait();   // see paged_rows.cu
+  pdl_trigger();
+  int item = blockIdx.x;
+  const int split = item % a.splits;
+  item /= a.splits;
+  const int block = item % a.blocks;
+  item /= a.blocks;
+  const int kh = item % p.K, who = item / p.K;
+  const int b0 = a.phase == kPrefix ? who * p.per : who;
+  const int rs = p.T * p.share;
+  const int rows = rs * (a.phase == kPrefix ? p.per : 1);
+  const int r0 = block * (a.two ? 256 : 128);
+  const Keys keys(p, a.phase, who);
+  // own keys that the block's last row sees
+  const int r_last = min(rows, r0 + (a.two ? 256 : 128)) - 1;
+  const int n_own = a.phase == kPrefix ? 0 : max(0, keys.n_own - p.T + r_last / p.share + 1);
+  const int nt_pre = (keys.n_pre + a.tile - 1) / a.tile, nt = nt_pre + (n_own + a.tile - 1) / a.tile;
+  const int per_split = (nt + a.splits - 1) / a.splits;
+  const int t0 = min(nt, split * per_split), n_tiles = min(nt, t0 + per_split) - t0;
+  // pipelines with work, and the consumers of a ring slot
+  const int pipes = n_tiles == 0 ? 0 : a.two ? (r0 + 128 < rows ? 2 : 1) : (n_tiles > 1 ? 2 : 1);
+  const int consumers = a.two ? pipes : 1;
+
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(smem_addr(&k_full[i]), 1);
+      mbar_init(smem_addr(&k_empty[i]), max(1, consumers));
+      mbar_init(smem_addr(&v_full[i]), 1);
+      mbar_init(smem_addr(&v_empty[i]), max(1, consumers));
+    }
+    for (int s = 0; s < 2; ++s) {
+      uint64_t* b = pipe_bars + 5 * s;
+      mbar_init(smem_addr(&b[0]), 4);
+      mbar_init(smem_addr(&b[1]), 1);
+      mbar_init(smem_addr(&b[2]), 4);
+      mbar_init(smem_addr(&b[3]), 4);
+      mbar_init(smem_addr(&b[4]), 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(tmem_slot)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  bool ok = true;
+
+  if (warp >= 10) {
+    // ------------------------------------------------ K (warp 10) and V (warp 11) copies, one lane per box
+    const bool is_v = warp == 11;
+    uint64_t *full = is_v ? v_full : k_full, *empty = is_v ? v_empty : k_empty;
+    uint8_t* ring = is_v ? sV : sK;
+    const CUtensorMap* map = is_v ? &tv : &tk;
+    // this lane's box of tile i: page id (-1: none) and slot
+    auto look = [&](int i, int& slot, int& boxes) -> int {
+      const int t = t0 + i;
+      const bool own = t >= nt_pre;
+      const int at = (own ? t - nt_pre : t) * a.tile, valid = min(a.tile, (own ? n_own : keys.n_pre) - at);
+      boxes = (valid + a.box - 1) / a.box;
+      if (lane >= boxes) return -1;
+      const int pos = at + lane * a.box;
+      slot = pos % p.page;
+      const int id = page_id((own ? keys.own : keys.pre)[pos / p.page], p.n_pages);
+      return id < 0 ? p.n_pages : id;   // past the pool: the map's fill value
+    };
+    int slot = 0, boxes = 0, id = n_tiles ? look(0, slot, boxes) : -1;
+    int i = 0;
+    for (; i < n_tiles && ok; ++i) {
+      const int st = i % ST;
+      int next_slot = 0, next_boxes = 0;
+      const int next = i + 1 < n_tiles ? look(i + 1, next_slot, next_boxes) : -1;
+      if (i >= ST && !mbar_wait(smem_addr(&empty[st]), (uint32_t)((i / ST - 1) & 1))) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) mbar_expect_tx(smem_addr(&full[st]), (uint32_t)(boxes * a.box * 128 * C::kPanels));
+      __syncwarp();
+      if (id >= 0) {
+        const uint32_t dst = smem_addr(ring + st * C::kTile) + (uint32_t)(lane * a.box * 128);
+#pragma unroll
+        for (int c = 0; c < C::kPanels; ++c)
+          tma_load_4d(dst + (uint32_t)(c * kPanel), map, smem_addr(&full[st]), c * 64, slot, kh, id);
+      }
+      id = next;
+      slot = next_slot;
+      boxes = next_boxes;
+    }
+    // given up: the copies in flight land before the CTA's shared memory goes
+    if (!ok)
+      for (int j = max(0, i - ST); j < i; ++j) mbar_wait(smem_addr(&full[j % ST]), (uint32_t)((j / ST) & 1));
+  } else if (warp >= 8) {
+    // ------------------------------------------------ MMA issue, one lane per pipeline
+    const int pipe = warp - 8;
+    if (lane == 0 && pipe < pipes) {
+      uint64_t* pb = pipe_bars + 5 * pipe;
+      const uint32_t tm = *tmem_slot + (uint32_t)(pipe * 256);
+      constexpr uint32_t idS = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+      constexpr uint32_t idO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
+                               ((uint32_t)(128 >> 4) << 24);
+      const int step = a.two ? 1 : 2, first = a.two ? 0 : pipe;
+      const uint64_t qd = desc_sw128(smem_addr(sQ + (a.two ? pipe : 0) * C::kTile));
+      if (!mbar_wait(smem_addr(&pipe_bars[a.two ? 5 * pipe : 0]), 0)) ok = false;
+      auto issue_s = [&](int i, int g) {   // tile i, the pipeline's g-th
+        const int st = i % ST;
+        if (ok && !mbar_wait(smem_addr(&k_full[st]), (uint32_t)((i / ST) & 1))) ok = false;
+        if (!C::kAlias && ok && g > 0 && !mbar_wait(smem_addr(&pb[2]), (uint32_t)((g - 1) & 1))) ok = false;
+        if (ok) {
+          tc_fence_after();
+          const uint64_t kd = desc_sw128(smem_addr(sK + st * C::kTile));
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t o = (uint64_t)((k / 4) * (kPanel >> 4) + (k % 4) * 2);
+            tc_mma(tm, qd + o, kd + o, idS, k > 0);
+          }
+        }
+        tc_commit(smem_addr(&pb[1]));
+        tc_commit(smem_addr(&k_empty[st]));
+      };
+      issue_s(first, 0);
+      int g = 0;
+      for (int i = first; i < n_tiles; i += step, ++g) {
+        if (!C::kAlias && i + step < n_tiles) issue_s(i + step, g + 1);
+        if (ok && !mbar_wait(smem_addr(&pb[3]), (uint32_t)(g & 1))) ok = false;
+        const int st = i % ST;
+        if (ok && !mbar_wait(smem_addr(&v_full[st]), (uint32_t)((i / ST) & 1))) ok = false;
+        if (ok) {
+          tc_fence_after();
+          const int t = t0 + i;
+          const int valid = min(a.tile, t < nt_pre ? keys.n_pre - t * a.tile : n_own - (t - nt_pre) * a.tile);
+          // MN-major: the leading byte offset is the distance of the 64-column panels
+          const uint64_t vd = desc_sw128(smem_addr(sV + st * C::kTile)) + ((uint64_t)((kPanel >> 4) - 1) << 16);
+          for (int k = 0; k < (valid + 15) / 16; ++k)   // 16 keys: 8 columns of packed P, 2 KB of V rows
+            tc_mma_ts(tm + C::kO, tm + C::kP + (uint32_t)(k * 8), vd + (uint64_t)(k * 128), idO, (g > 0 || k > 0) ? 1u : 0u);
+        }
+        tc_commit(smem_addr(&pb[4]));
+        tc_commit(smem_addr(&v_empty[st]));
+        if (C::kAlias && i + step < n_tiles) issue_s(i + step, g + 1);
+      }
+    }
+  } else {
+    // ------------------------------------------------ softmax: thread = row = TMEM lane
+    const int pipe = warp >> 2, rl = tid & 127;
+    uint64_t* pb = pipe_bars + 5 * pipe;
+    const int r = r0 + (a.two ? pipe * 128 : 0) + rl;
+    const bool live = r < rows;
+    const int b = b0 + (live ? r / rs : 0), rr = live ? r % rs : 0, t = rr / p.share, h = kh * p.share + rr % p.share;
+    // Q into its tile (with two == 0 by pipeline 0 for both)
+    if (pipes > 0 && (pipe == 0 || a.two)) {
+      uint8_t* dst = sQ + (a.two ? pipe : 0) * C::kTile + rl * 128;
+      const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + b * p.q_b + (int64_t)h * p.q_h + t * p.q_t);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c)
+        *reinterpret_cast<uint4*>(dst + (c / 8) * kPanel + (((c & 7) ^ (rl & 7)) << 4)) = live ? src[c] : uint4{};
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_addr(&pb[0]));
+    }
+    const uint32_t tm = *tmem_slot + (uint32_t)(pipe * 256) + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t tS = tm, tP = tm + C::kP, tO = tm + C::kO;
+    const int last = a.phase == kPrefix ? 0 : keys.n_own - p.T + t;   // last own key of the row; below 0: padding
+    const int seen_own = live ? max(0, last + 1) : 0;
+    const int seen_pre = live && (a.phase == kPrefix || last >= 0) ? keys.n_pre : 0;
+    float m = -INFINITY, l = 0.f;
+    int g = 0;
+    if (pipe < pipes) {
+      const int step = a.two ? 1 : 2;
+      for (int i = a.two ? 0 : pipe; i < n_tiles; i += step, ++g) {
+        const int tt = t0 + i;
+        const bool own = tt >= nt_pre;
+        const int at = (own ? tt - nt_pre : tt) * a.tile;
+        const int nvalid = min(a.tile, (own ? seen_own : seen_pre) - at);   // of this row
+        const int valid = min(a.tile, (own ? n_own : keys.n_pre) - at);     // of the tile
+        if (ok && !mbar_wait(smem_addr(&pb[1]), (uint32_t)(g & 1))) ok = false;
+        tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) tmem_ld32_nw(tS + (uint32_t)c, s + c);
+        tmem_wait_ld();
+        if (!C::kAlias) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_addr(&pb[2]));
+        }
+        if (nvalid < 128) {
+#pragma unroll
+          for (int k = 0; k < 128; ++k)
+            if (k >= nvalid) s[k] = 0xff800000u;   // -inf: exponential 0
+        }
+        float m8[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 8]));
+#pragma unroll
+        for (int k = 16; k < 128; k += 16)
+#pragma unroll
+          for (int c = 0; c < 8; ++c) m8[c] = fmax3(m8[c], __uint_as_float(s[k + c]), __uint_as_float(s[k + 8 + c]));
+        float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
+        mx *= p.scale_log2;
+        bool rescale = false;
+        float alpha = 1.f;
+        if (g == 0) {
+          m = mx;
+        } else if (mx > m + kTcRescale) {   // also from m = -inf, no keys so far
+          alpha = ex2(m - mx);
+          m = mx;
+          rescale = true;
+        }
+        // P's columns and O are free once the PV before has completed (aliased: before this S)
+        if (!C::kAlias && g > 0) {
+          if (ok && !mbar_wait(smem_addr(&pb[4]), (uint32_t)((g - 1) & 1))) ok = false;
+          tc_fence_after();
+        }
+        const float from = m == -INFINITY ? 0.f : m;
+        const uint64_t sc2 = pack_f2(p.scale_log2, p.scale_log2), nm2 = pack_f2(-from, -from);
+        uint64_t acc2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t w[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            float x0, x1;
+            unpack_f2(ffma2(pack_u2(s[c + 2 * k], s[c + 2 * k + 1]), sc2, nm2), x0, x1);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            acc2[k & 1] = fadd2(acc2[k & 1], pack_f2(p0, p1));
+            w[k] = tc::pack2_bf16(p0, p1);
+          }
+          tmem_st16(tP + (uint32_t)(c / 2), w);
+        }
+        float s0, s1, s2, s3;
+        unpack_f2(acc2[0], s0, s1);
+        unpack_f2(acc2[1], s2, s3);
+        if (__any_sync(0xffffffffu, rescale)) {   // whole warp: tcgen05.ld / st are warp-wide
+          uint32_t o[32];
+#pragma unroll
+          for (int c = 0; c < D; c += 32) {
+            tmem_ld32(tO + (uint32_t)c, o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(tO + (uint32_t)c, o);
+          }
+          l *= alpha;
+        }
+        l += (s0 + s1) + (s2 + s3);
+        tmem_wait_st();
+        if (valid & 15) {   // the last step's V rows behind the keys
+          const int st = i % ST;
+          if (ok && !mbar_wait(smem_addr(&v_full[st]), (uint32_t)((i / ST) & 1))) ok = false;
+          const int clear = 16 - (valid & 15);
+          for (int k = rl; k < clear * 8 * C::kPanels; k += 128)
+            *reinterpret_cast<uint4*>(sV + st * C::kTile + (k / (clear * 8)) * kPanel + valid * 128 + (k % (clear * 8)) * 16) =
+                uint4{};
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&pb[3]));
+      }
+      if (ok && !mbar_wait(smem_addr(&pb[4]), (uint32_t)((g - 1) & 1))) ok = false;
+      tc_fence_after();
+    }
+    // the row's result: out, or its slot of partial results
+    if (a.early) pdl_wait();
+    const int64_t row = row_id(p, b, t, h);
+    const int64_t slot = (int64_t)a.slot0 + (a.two ? split : 2 * split + pipe);
+    const int64_t at = slot * p.B * p.T * p.H + row;
+    const bool mine = live && (a.direct ? a.two != 0 || pipe == 0 : true);
+    const bool none = l == 0.f;
+    if (mine && !a.direct) p.ml[at] = make_float2(m, l);
+    const float inv = none ? 0.f : 1.f / l;
+    if (pipe < pipes) {
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        tmem_ld32(tO + (uint32_t)c, o);
+        if (!mine) continue;
+        if (a.direct) {
+          uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + c);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              w[u] = none ? 0u : tc::pack2_bf16(__uint_as_float(o[8 * k + 2 * u]) * inv, __uint_as_float(o[8 * k + 2 * u + 1]) * inv);
+            dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        } else if (!none) {
+          uint4* dst = reinterpret_cast<uint4*>(p.acc + at * D + c);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+    } else if (mine && a.direct) {   // no keys at all: rows of padding
+      uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)p.out + b * p.o_b + h * p.o_h + t * p.o_t);
+#pragma unroll
+      for (int k = 0; k < D / 8; ++k) dst[k] = uint4{};
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(*tmem_slot), "r"(512u));
+  }
+}
+
+// Whether the kernel serves the call: head size, pages that make tiles of whole 8-row swizzle atoms, 16-byte rows.
+static bool tc_eligible(const Attn& p) {
+  if (p.D != 64 && p.D != 128) return false;
+  if (p.page % 8 || (p.page > 128 && p.page % 128)) return false;
+  for (const void* x : {p.q, (const void*)p.out, p.k, p.v})
+    if (!aligned(x, 16)) return false;
+  for (int64_t s : {p.page_stride, p.head_stride, p.slot_stride})
+    if (s % 8 || s <= 0 || s >= (1LL << 38)) return false;
+  for (int64_t s : {p.q_b, p.q_h, p.q_t, p.o_b, p.o_h, p.o_t})
+    if (s % 8) return false;
+  return true;
+}
+
+static int page_map(CUtensorMap* map, const void* pages, const Attn& p, int box) {
+  auto enc = tc::get_encode();
+  if (!enc) return fail(GPT_ERR_CUDA, "cuTensorMapEncodeTiled unavailable from the driver");
+  cuuint64_t dims[4] = {(cuuint64_t)p.D, (cuuint64_t)p.page, (cuuint64_t)p.K, (cuuint64_t)p.n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)p.slot_stride * 2, (cuuint64_t)p.head_stride * 2, (cuuint64_t)p.page_stride * 2};
+  cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pages), dims, strides, boxes, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GPT_ERR_CUDA, "cuTensorMapEncodeTiled (paged cache) failed (%d)", (int)r);
+  return GPT_OK;
+}
+
+template <int D>
+static int launch_tc_d(const Attn& p, TcArgs a, cudaStream_t st) {
+  static bool done[64] = {false};
+  static std::mutex mu;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> g(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<D>::kSmem);
+      if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      done[dev] = true;
+    }
+  }
+  a.box = p.page < 128 ? p.page : 128;
+  a.tile = 128 / a.box * a.box;
+  CUtensorMap mk, mv;
+  int s = page_map(&mk, p.k, p, a.box);
+  if (!s) s = page_map(&mv, p.v, p, a.box);
+  if (s) return s;
+  const int64_t rows = (int64_t)p.T * p.share * (a.phase == kPrefix ? p.per : 1), block = a.two ? 256 : 128;
+  const int64_t blocks = (rows + block - 1) / block;
+  const int64_t grid = blocks * a.splits * p.K * (a.phase == kPrefix ? p.B / p.per : p.B);
+  GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
+  a.blocks = (int)blocks;
+  launch_pdl(paged_tc_kernel<D>, dim3((unsigned)grid), dim3(kTcThreads), Tc<D>::kSmem, st, mk, mv, p, a);
+  return launch_status("paged_tc");
+}
+
+static int launch_tc(const Attn& p, const TcArgs& a, cudaStream_t st) {
+  return p.D == 64 ? launch_tc_d<64>(p, a, st) : launch_tc_d<128>(p, a, st);
+}
+
+}  // namespace paged
+}  // namespace gpt
