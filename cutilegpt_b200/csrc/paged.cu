@@ -66,7 +66,9 @@ static int shares(int64_t items, int64_t keys, int sms, int per_sm, int64_t leas
 
 static void plan_launch(Kernel kernel, int64_t rows, int64_t items, int64_t keys, int sms, int* splits, int* two,
                         int* slots) {
-  *two = kernel == kTc && rows > 128;
+  // 256 rows on the same tiles, but for three 128-row blocks, which two pipelines of their own serve in 1.5 passes, not 2
+  const int64_t tiles128 = (rows + 127) / 128;
+  *two = kernel == kTc && tiles128 > 1 && tiles128 != 3;
   if (kernel == kTc) {
     // one CTA on an SM: no more than fit at once, at least two tiles for a pipeline
     items *= (rows + (*two ? 255 : 127)) / (*two ? 256 : 128);

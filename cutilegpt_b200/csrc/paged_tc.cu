@@ -18,8 +18,10 @@
 //   O += P V      A = P from TMEM, B = V MN-major as its boxes arrive; only the 16-key steps
 //                 that hold keys are issued, and the last one's rows behind the keys are cleared
 //                 first: what the cache holds there must not meet P = 0
-// m moves only when a tile's maximum exceeds it by 2^8 (then O and the sum are
-// rescaled), so P stays below 2^8 and O / l is the same softmax. With D = 64 P has
+// The exponentials do not wait for the tile's maximum: m is what earlier tiles left,
+// P = 2^(s - m) may exceed 1 (fp32 and bf16 have the range), a tile whose maximum lies 2^8 above m
+// makes the next tile move m (O and the sum are rescaled), one 2^64 above moves it at once and
+// starts over. The PV of a tile's first 64 keys runs under the exponentials of the others. With D = 64 P has
 // TMEM columns of its own and the next S is computed under the softmax; with D = 128
 // P takes the place of S (256 columns a pipeline), and the next S follows the PV.
 // Keys and values have separate rings; every wait is bounded.
@@ -56,7 +58,8 @@ using tc::tmem_ld32;
 
 constexpr int kTcThreads = 12 * 32;      // 2 x 4 softmax warps, 2 MMA warps, K and V copy warps
 constexpr int kPanel = 128 * 128;        // 128 rows of 64 bf16, 128-byte swizzled
-constexpr float kTcRescale = 8.f;        // log2 of the largest P before O is rescaled
+constexpr float kTcRescale = 8.f;        // log2 of the P from which the next tile moves m
+constexpr float kTcFar = 64.f;           // log2 of the P from which the tile itself moves m and starts over
 
 template <int D>
 struct Tc {
@@ -87,8 +90,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
   uint8_t* sV = sK + ST * C::kTile;         // [ST][kTile]
   uint64_t* bars = (uint64_t*)(sV + ST * C::kTile);
   uint64_t *k_full = bars, *k_empty = bars + ST, *v_full = bars + 2 * ST, *v_empty = bars + 3 * ST;
-  uint64_t* pipe_bars = bars + 4 * ST;      // per pipeline: q_full, s_full, s_free, p_full, o_full
-  uint32_t* tmem_slot = (uint32_t*)(pipe_bars + 10);
+  uint64_t* pipe_bars = bars + 4 * ST;      // per pipeline: q_full, s_full, s_free, p_full (two halves), o_full
+  uint64_t* turns = pipe_bars + 12;         // [pipeline][warp of the warpgroup]: its exponentials may begin
+  uint32_t* tmem_slot = (uint32_t*)(turns + 8);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (!a.early) pdl_wait();   // see paged_rows.cu
@@ -122,13 +126,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       mbar_init(smem_addr(&v_empty[i]), max(1, consumers));
     }
     for (int s = 0; s < 2; ++s) {
-      uint64_t* b = pipe_bars + 5 * s;
+      uint64_t* b = pipe_bars + 6 * s;
       mbar_init(smem_addr(&b[0]), 4);
       mbar_init(smem_addr(&b[1]), 1);
       mbar_init(smem_addr(&b[2]), 4);
       mbar_init(smem_addr(&b[3]), 4);
-      mbar_init(smem_addr(&b[4]), 1);
+      mbar_init(smem_addr(&b[4]), 4);
+      mbar_init(smem_addr(&b[5]), 1);
     }
+    for (int i = 0; i < 8; ++i) mbar_init(smem_addr(&turns[i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -188,55 +194,76 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     // ------------------------------------------------ MMA issue, one lane per pipeline
     const int pipe = warp - 8;
     if (lane == 0 && pipe < pipes) {
-      uint64_t* pb = pipe_bars + 5 * pipe;
+      uint64_t* pb = pipe_bars + 6 * pipe;
       const uint32_t tm = *tmem_slot + (uint32_t)(pipe * 256);
       constexpr uint32_t idS = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(128 >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
       constexpr uint32_t idO = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
                                ((uint32_t)(128 >> 4) << 24);
       const int step = a.two ? 1 : 2, first = a.two ? 0 : pipe;
+      // The lane's own instructions stand between a tile's softmax and its products, so what they
+      // need is at hand before the waits: addresses, stage-0 descriptors, stages and parities.
+      const uint32_t s_full = smem_addr(&pb[1]), s_free = smem_addr(&pb[2]), p_half0 = smem_addr(&pb[3]),
+                     p_half1 = smem_addr(&pb[4]), o_full = smem_addr(&pb[5]);
+      const uint32_t kf = smem_addr(k_full), ke = smem_addr(k_empty), vf = smem_addr(v_full), ve = smem_addr(v_empty);
       const uint64_t qd = desc_sw128(smem_addr(sQ + (a.two ? pipe : 0) * C::kTile));
-      if (!mbar_wait(smem_addr(&pipe_bars[a.two ? 5 * pipe : 0]), 0)) ok = false;
-      auto issue_s = [&](int i, int g) {   // tile i, the pipeline's g-th
-        const int st = i % ST;
-        if (ok && !mbar_wait(smem_addr(&k_full[st]), (uint32_t)((i / ST) & 1))) ok = false;
-        if (!C::kAlias && ok && g > 0 && !mbar_wait(smem_addr(&pb[2]), (uint32_t)((g - 1) & 1))) ok = false;
-        if (ok) {
-          tc_fence_after();
-          const uint64_t kd = desc_sw128(smem_addr(sK + st * C::kTile));
+      const uint64_t kd0 = desc_sw128(smem_addr(sK));
+      // MN-major: the leading byte offset is the distance of the 64-column panels
+      const uint64_t vd0 = desc_sw128(smem_addr(sV)) + ((uint64_t)((kPanel >> 4) - 1) << 16);
+      int ks = first % ST, vs = ks;              // ring slots of the next S and the next PV
+      uint32_t kpar = 0, vpar = 0;
+      auto issue_s = [&](int g) {                // the pipeline's g-th tile
+        const uint64_t kd = kd0 + (uint64_t)(ks * (C::kTile >> 4));
+        if (!mbar_wait(kf + 8 * ks, kpar)) return false;
+        if (!C::kAlias && g > 0 && !mbar_wait(s_free, (uint32_t)((g - 1) & 1))) return false;
+        tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t o = (uint64_t)((k / 4) * (kPanel >> 4) + (k % 4) * 2);
-            tc_mma(tm, qd + o, kd + o, idS, k > 0);
-          }
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t o = (uint64_t)((k / 4) * (kPanel >> 4) + (k % 4) * 2);
+          tc_mma(tm, qd + o, kd + o, idS, k > 0);
         }
-        tc_commit(smem_addr(&pb[1]));
-        tc_commit(smem_addr(&k_empty[st]));
+        tc_commit(s_full);
+        tc_commit(ke + 8 * ks);
+        ks += step;
+        if (ks >= ST) ks -= ST, kpar ^= 1;
+        return true;
       };
-      issue_s(first, 0);
+      ok = mbar_wait(smem_addr(&pipe_bars[a.two ? 6 * pipe : 0]), 0) && issue_s(0);
       int g = 0;
-      for (int i = first; i < n_tiles; i += step, ++g) {
-        if (!C::kAlias && i + step < n_tiles) issue_s(i + step, g + 1);
-        if (ok && !mbar_wait(smem_addr(&pb[3]), (uint32_t)(g & 1))) ok = false;
-        const int st = i % ST;
-        if (ok && !mbar_wait(smem_addr(&v_full[st]), (uint32_t)((i / ST) & 1))) ok = false;
-        if (ok) {
-          tc_fence_after();
-          const int t = t0 + i;
-          const int valid = min(a.tile, t < nt_pre ? keys.n_pre - t * a.tile : n_own - (t - nt_pre) * a.tile);
-          // MN-major: the leading byte offset is the distance of the 64-column panels
-          const uint64_t vd = desc_sw128(smem_addr(sV + st * C::kTile)) + ((uint64_t)((kPanel >> 4) - 1) << 16);
-          for (int k = 0; k < (valid + 15) / 16; ++k)   // 16 keys: 8 columns of packed P, 2 KB of V rows
-            tc_mma_ts(tm + C::kO, tm + C::kP + (uint32_t)(k * 8), vd + (uint64_t)(k * 128), idO, (g > 0 || k > 0) ? 1u : 0u);
+      for (int i = first; ok && i < n_tiles; i += step, ++g) {
+        const int t = t0 + i;
+        const int valid = min(a.tile, t < nt_pre ? keys.n_pre - t * a.tile : n_own - (t - nt_pre) * a.tile);
+        const int steps = (valid + 15) / 16;     // 16 keys: 8 columns of packed P, 2 KB of V rows
+        const uint64_t vd = vd0 + (uint64_t)(vs * (C::kTile >> 4));
+        const bool more = i + step < n_tiles;
+        if (!C::kAlias && more && !(ok = issue_s(g + 1))) break;
+        if (!(ok = mbar_wait(vf + 8 * vs, vpar) && mbar_wait(p_half0, (uint32_t)(g & 1)))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (k < steps) tc_mma_ts(tm + C::kO, tm + C::kP + (uint32_t)(k * 8), vd + (uint64_t)(k * 128), idO, (k > 0 || g > 0) ? 1u : 0u);
+        if (!(ok = mbar_wait(p_half1, (uint32_t)(g & 1)))) break;
+        tc_fence_after();
+        if (steps == 8) {
+#pragma unroll
+          for (int k = 4; k < 8; ++k) tc_mma_ts(tm + C::kO, tm + C::kP + (uint32_t)(k * 8), vd + (uint64_t)(k * 128), idO, 1u);
+        } else {
+          for (int k = 4; k < steps; ++k) tc_mma_ts(tm + C::kO, tm + C::kP + (uint32_t)(k * 8), vd + (uint64_t)(k * 128), idO, 1u);
         }
-        tc_commit(smem_addr(&pb[4]));
-        tc_commit(smem_addr(&v_empty[st]));
-        if (C::kAlias && i + step < n_tiles) issue_s(i + step, g + 1);
+        if (C::kAlias && more) {                 // the arrival of the next S says that this PV is done
+          tc_commit(ve + 8 * vs);
+          if (!(ok = issue_s(g + 1))) break;
+        } else {
+          tc_commit(o_full);
+          tc_commit(ve + 8 * vs);
+        }
+        vs += step;
+        if (vs >= ST) vs -= ST, vpar ^= 1;
       }
     }
   } else {
     // ------------------------------------------------ softmax: thread = row = TMEM lane
     const int pipe = warp >> 2, rl = tid & 127;
-    uint64_t* pb = pipe_bars + 5 * pipe;
+    uint64_t* pb = pipe_bars + 6 * pipe;
     const int r = r0 + (a.two ? pipe * 128 : 0) + rl;
     const bool live = r < rows;
     const int b = b0 + (live ? r / rs : 0), rr = live ? r % rs : 0, t = rr / p.share, h = kh * p.share + rr % p.share;
@@ -256,9 +283,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     const int last = a.phase == kPrefix ? 0 : keys.n_own - p.T + t;   // last own key of the row; below 0: padding
     const int seen_own = live ? max(0, last + 1) : 0;
     const int seen_pre = live && (a.phase == kPrefix || last >= 0) ? keys.n_pre : 0;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, top = -INFINITY;   // top: the largest scaled score so far
     int g = 0;
     if (pipe < pipes) {
+      const uint64_t sc2 = pack_f2(p.scale_log2, p.scale_log2);
       const int step = a.two ? 1 : 2;
       for (int i = a.two ? 0 : pipe; i < n_tiles; i += step, ++g) {
         const int tt = t0 + i;
@@ -269,61 +297,82 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         if (ok && !mbar_wait(smem_addr(&pb[1]), (uint32_t)(g & 1))) ok = false;
         tc_fence_after();
         uint32_t s[128];
+        auto load = [&](int n) {   // the first n scores, -inf for what the row does not see
 #pragma unroll
-        for (int c = 0; c < 128; c += 32) tmem_ld32_nw(tS + (uint32_t)c, s + c);
-        tmem_wait_ld();
+          for (int c = 0; c < n; c += 32) tmem_ld32_nw(tS + (uint32_t)c, s + c);
+          tmem_wait_ld();
+          if (nvalid < n) {
+#pragma unroll
+            for (int k = 0; k < n; ++k)
+              if (k >= nvalid) s[k] = 0xff800000u;
+          }
+        };
+        load(128);
+        auto row_max = [&]() {
+          float m8[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 8]));
+#pragma unroll
+          for (int k = 16; k < 128; k += 16)
+#pragma unroll
+            for (int c = 0; c < 8; ++c) m8[c] = fmax3(m8[c], __uint_as_float(s[k + c]), __uint_as_float(s[k + 8 + c]));
+          return fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * p.scale_log2;
+        };
+        bool rescale = false;
+        float alpha = 1.f;
+        auto move_to = [&](float to) {   // also from m = -inf, no keys so far
+          const float f = ex2(m - to);
+          alpha *= f;
+          l *= f;
+          m = to;
+          rescale = g > 0;
+        };
+        if (g == 0)
+          m = row_max();
+        else if (top > m + kTcRescale)
+          move_to(top);
+        // The two warps of a scheduler take turns at the exponentials, pipeline 0 first: while one's fill
+        // the special-function unit the other's products run. Left alone the pipelines fall into step
+        // and neither overlaps the other.
+        if (pipes == 2 && (pipe == 1 || g > 0)) {
+          if (ok && !mbar_wait(smem_addr(&turns[warp]), (uint32_t)((pipe == 1 ? g : g - 1) & 1))) ok = false;
+        }
+        uint64_t sum2[2];
+        uint32_t w[32];
+        // 64 keys from column c on: P into w, their sum
+        auto exps = [&](int c, bool fresh) {
+          const float from = m == -INFINITY ? 0.f : m;
+          const uint64_t nm2 = pack_f2(-from, -from);
+          if (fresh) sum2[0] = sum2[1] = 0ull;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            float x0, x1;
+            unpack_f2(ffma2(pack_u2(s[c + 2 * k], s[c + 2 * k + 1]), sc2, nm2), x0, x1);
+            const float p0 = ex2(x0), p1 = ex2(x1);
+            sum2[k & 1] = fadd2(sum2[k & 1], pack_f2(p0, p1));
+            w[k] = tc::pack2_bf16(p0, p1);
+          }
+        };
+        exps(0, true);
+        const float mx = row_max();   // beside the exponentials
+        if (__any_sync(0xffffffffu, mx > m + kTcFar)) {
+          if (mx > m + kTcFar) move_to(mx);
+          load(64);
+          exps(0, true);
+        }
+        top = mx;
         if (!C::kAlias) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_addr(&pb[2]));
         }
-        if (nvalid < 128) {
-#pragma unroll
-          for (int k = 0; k < 128; ++k)
-            if (k >= nvalid) s[k] = 0xff800000u;   // -inf: exponential 0
-        }
-        float m8[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m8[k] = fmaxf(__uint_as_float(s[k]), __uint_as_float(s[k + 8]));
-#pragma unroll
-        for (int k = 16; k < 128; k += 16)
-#pragma unroll
-          for (int c = 0; c < 8; ++c) m8[c] = fmax3(m8[c], __uint_as_float(s[k + c]), __uint_as_float(s[k + 8 + c]));
-        float mx = fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7]));
-        mx *= p.scale_log2;
-        bool rescale = false;
-        float alpha = 1.f;
-        if (g == 0) {
-          m = mx;
-        } else if (mx > m + kTcRescale) {   // also from m = -inf, no keys so far
-          alpha = ex2(m - mx);
-          m = mx;
-          rescale = true;
-        }
         // P's columns and O are free once the PV before has completed (aliased: before this S)
         if (!C::kAlias && g > 0) {
-          if (ok && !mbar_wait(smem_addr(&pb[4]), (uint32_t)((g - 1) & 1))) ok = false;
+          if (ok && !mbar_wait(smem_addr(&pb[5]), (uint32_t)((g - 1) & 1))) ok = false;
           tc_fence_after();
         }
-        const float from = m == -INFINITY ? 0.f : m;
-        const uint64_t sc2 = pack_f2(p.scale_log2, p.scale_log2), nm2 = pack_f2(-from, -from);
-        uint64_t acc2[2] = {0ull, 0ull};
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) {
-          uint32_t w[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            float x0, x1;
-            unpack_f2(ffma2(pack_u2(s[c + 2 * k], s[c + 2 * k + 1]), sc2, nm2), x0, x1);
-            const float p0 = ex2(x0), p1 = ex2(x1);
-            acc2[k & 1] = fadd2(acc2[k & 1], pack_f2(p0, p1));
-            w[k] = tc::pack2_bf16(p0, p1);
-          }
-          tmem_st16(tP + (uint32_t)(c / 2), w);
-        }
-        float s0, s1, s2, s3;
-        unpack_f2(acc2[0], s0, s1);
-        unpack_f2(acc2[1], s2, s3);
+        tmem_st16(tP, w);
+        tmem_st16(tP + 16, w + 16);
         if (__any_sync(0xffffffffu, rescale)) {   // whole warp: tcgen05.ld / st are warp-wide
           uint32_t o[32];
 #pragma unroll
@@ -333,10 +382,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
             for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
             tmem_st32(tO + (uint32_t)c, o);
           }
-          l *= alpha;
         }
-        l += (s0 + s1) + (s2 + s3);
-        tmem_wait_st();
         if (valid & 15) {   // the last step's V rows behind the keys
           const int st = i % ST;
           if (ok && !mbar_wait(smem_addr(&v_full[st]), (uint32_t)((i / ST) & 1))) ok = false;
@@ -346,11 +392,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
                 uint4{};
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
+        tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&pb[3]));
+        if (lane == 0) mbar_arrive(smem_addr(&pb[3]));   // the PV of the first 64 keys may run
+        exps(64, false);
+        tmem_st16(tP + 32, w);
+        tmem_st16(tP + 48, w + 16);
+        // the turn passes on behind the stores: without them the compiler moves the exponentials past it
+        __syncwarp();
+        if (pipes == 2 && lane == 0) mbar_arrive(smem_addr(&turns[warp ^ 4]));
+        float s0, s1, s2, s3;
+        unpack_f2(sum2[0], s0, s1);
+        unpack_f2(sum2[1], s2, s3);
+        l += (s0 + s1) + (s2 + s3);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&pb[4]));
       }
-      if (ok && !mbar_wait(smem_addr(&pb[4]), (uint32_t)((g - 1) & 1))) ok = false;
+      // the last PV: with aliased P the only one that arrives here
+      if (ok && !mbar_wait(smem_addr(&pb[5]), C::kAlias ? 0u : (uint32_t)((g - 1) & 1))) ok = false;
       tc_fence_after();
     }
     // the row's result: out, or its slot of partial results
