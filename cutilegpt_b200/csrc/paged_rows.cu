@@ -20,15 +20,19 @@ namespace gpt {
 namespace paged {
 
 constexpr int kRowTile = 16;
-constexpr int kRowWarps = 4;
-constexpr int kRing = 3;
 
-// Keys of a warp's step: 8 KB of keys and values, at most 64 keys.
-constexpr int step_keys(int dp) { return 2048 / dp < 64 ? 2048 / dp : 64; }
-constexpr int rows_smem(int dp) {
-  const int ring = kRowWarps * kRing * step_keys(dp) * dp * 4, merge = kRowWarps * kRowTile * (dp + 4) * 4;
-  return ring > merge ? ring : merge;
-}
+template <int DP, int W>   // W warps
+struct Rows {
+  static constexpr int kKeys = DP >= 64 ? 16 : 1024 / DP;      // keys of a warp's step
+  static constexpr int kTile = kKeys * DP * 2;                 // bytes of a step's keys
+  static constexpr int kRing = DP == 128 ? 2 : 3;              // steps of a warp's ring
+  static constexpr int kCtas = (DP == 128 ? 12 : 16) / W;      // of an SM
+  static constexpr bool kQShared = DP == 128;                  // Q fragments are read from shared memory at every step
+  static constexpr int kRings = W * kRing * 2 * kTile;
+  static constexpr int kMerge = W * kRowTile * (DP + 2) * 4;
+  static constexpr int kQ = kQShared ? kRowTile * DP * 2 : 0;
+  static constexpr int kSmem = (kRings > kMerge ? kRings : kMerge) + kQ;
+};
 
 // Byte offset of 16-byte chunk c of row r in a tile of rows of DP bf16, chunks permuted
 // inside a row so that eight consecutive rows of one chunk column hit eight bank groups.
@@ -65,39 +69,46 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// One row's four columns joined with the partial slots first .. first + n - 1.
+// One row's four columns joined with the partial slots first .. first + n - 1, eight at a time.
 __device__ __forceinline__ void join4(const Attn& p, int first, int n, int64_t row, int d, float& m, float& l, float4& acc) {
   const int64_t rows = (int64_t)p.B * p.T * p.H;
-  const float2* ml = p.ml + first * rows + row;
-  float top = l == 0.f ? -INFINITY : m;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float2 o = ml[s * rows];
-    if (o.y != 0.f) top = fmaxf(top, o.x);
-  }
-  const float a = l == 0.f ? 0.f : exp2f(m - top);
-  m = top;
-  l *= a;
-  acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
-#pragma unroll 4
-  for (int s = 0; s < n; ++s) {
-    const float2 o = ml[s * rows];
-    if (o.y == 0.f) continue;   // no keys: its accumulator was not written
-    const float w = exp2f(o.x - top);
-    const float4 v = *reinterpret_cast<const float4*>(p.acc + ((int64_t)(first + s) * rows + row) * p.D + d);
-    l = fmaf(o.y, w, l);
-    acc.x = fmaf(v.x, w, acc.x);
-    acc.y = fmaf(v.y, w, acc.y);
-    acc.z = fmaf(v.z, w, acc.z);
-    acc.w = fmaf(v.w, w, acc.w);
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    float2 o[8];
+    float4 v[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const int64_t at = (int64_t)(first + min(s0 + s, n - 1)) * rows + row;
+      o[s] = __ldcg(p.ml + at);
+      v[s] = __ldcg(reinterpret_cast<const float4*>(p.acc + at * p.D + d));
+      if (s0 + s >= n) o[s].y = 0.f;
+    }
+    float top = l == 0.f ? -INFINITY : m;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (o[s].y != 0.f) top = fmaxf(top, o[s].x);
+    const float a = l == 0.f ? 0.f : exp2f(m - top);
+    m = top;
+    l *= a;
+    acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if (o[s].y == 0.f) continue;   // no keys: its accumulator was not written
+      const float w = exp2f(o[s].x - top);
+      l = fmaf(o[s].y, w, l);
+      acc.x = fmaf(v[s].x, w, acc.x);
+      acc.y = fmaf(v[s].y, w, acc.y);
+      acc.z = fmaf(v[s].z, w, acc.z);
+      acc.w = fmaf(v[s].w, w, acc.w);
+    }
   }
 }
 
-template <int DP>
-__global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Attn p, int phase, int splits, int blocks,
-                                                                       int slot0, int direct, int early) {
-  constexpr int KS = step_keys(DP), kChunks = DP / 8, kLoads = KS * kChunks / 32;
-  constexpr int kTile = KS * DP * 2;                  // bytes of a step's keys
+template <int DP, int W>
+__global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kernel(const Attn p, int phase, int splits,
+                                                                                  int blocks, int slot0, int direct,
+                                                                                  int early) {
+  using C = Rows<DP, W>;
+  constexpr int KS = C::kKeys, kChunks = DP / 8, kLoads = KS * kChunks / 32, kTile = C::kTile, kRing = C::kRing;
   extern __shared__ __align__(128) uint8_t rows_smem_dyn[];
   // With `early` the launch before is this call's prefix launch, whose every CTA has waited for all
   // that came before it: what is read and written here is then safe, but for the prefix's partial results.
@@ -122,8 +133,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
 
   // Q in the A fragments: rows lane / 4 and lane / 4 + 8
   uint32_t qf[DP / 16][4];
-  int seen[2];        // keys below this one are the row's
-  int most = 0;       // largest of the tile's
+  int seen[2];                      // keys below this one are the row's
+  int most = 0, least = n;          // the largest and the smallest of the tile's
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = r0 + lane / 4 + 8 * half;
@@ -132,6 +143,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
     seen[half] = !live ? 0 : phase == kPrefix ? n : max(0, keys.n_pre + keys.n_own - p.T + t + 1);
     if (live && phase != kPrefix && keys.n_own - p.T + t < 0) seen[half] = 0;   // padding sees nothing
     most = max(most, seen[half]);
+    if (live) least = min(least, seen[half]);
     const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + b * p.q_b + (int64_t)(kh * p.share + rr % p.share) * p.q_h + t * p.q_t;
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k)
@@ -142,20 +154,29 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
       }
   }
   j1 = min(j1, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
+  least = min(j1, (int)__reduce_min_sync(0xffffffffu, (unsigned)least));
 
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem_dyn) + warp * (kRing * 2 * kTile);
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem_dyn) + C::kQ + warp * (kRing * 2 * kTile);
   if (p.D < DP) {   // columns behind D stay zeros
-    for (int i = threadIdx.x; i < rows_smem(DP) / 16; i += blockDim.x) reinterpret_cast<uint4*>(rows_smem_dyn)[i] = uint4{};
+    for (int i = threadIdx.x; i < C::kRings / 16; i += blockDim.x) reinterpret_cast<uint4*>(rows_smem_dyn + C::kQ)[i] = uint4{};
     __syncthreads();
   }
-  const int steps = j1 > j0 + warp * KS ? (j1 - j0 - warp * KS + kRowWarps * KS - 1) / (kRowWarps * KS) : 0;
+  uint4* sq = reinterpret_cast<uint4*>(rows_smem_dyn);   // with kQShared: the fragments, [k][lane]
+  if (C::kQShared) {
+    if (warp == 0) {
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) sq[k * 32 + lane] = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
+    }
+    __syncthreads();
+  }
+  const int steps = j1 > j0 + warp * KS ? (j1 - j0 - warp * KS + W * KS - 1) / (W * KS) : 0;
   // lane i holds the offsets of keys i, i + 32, ... of a step, -1 where there is none
   constexpr int kOffs = (KS + 31) / 32;
   int64_t off[kOffs];
   auto locate = [&](int s) {
 #pragma unroll
     for (int i = 0; i < kOffs; ++i) {
-      const int in = lane + 32 * i, j = j0 + (s * kRowWarps + warp) * KS + in;
+      const int in = lane + 32 * i, j = j0 + (s * W + warp) * KS + in;
       off[i] = in < KS && s < steps && j < j1 ? keys.offset(p, j, kh) : -1;
     }
   };
@@ -191,45 +212,62 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
     fetch(s + kRing - 1);      // into the slot of step s - 1, which every lane has left
     locate(s + kRing);         // the table read is on its way while this step computes
     const uint32_t sk = ring + (uint32_t)(s % kRing) * (2 * kTile), sv = sk + kTile;
-    const int j = j0 + (s * kRowWarps + warp) * KS;
+    const int j = j0 + (s * W + warp) * KS;
     float sc[KS / 8][4];
 #pragma unroll
     for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) sc[i][k] = 0.f;
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
+    for (int k = 0; k < DP / 16; ++k) {
+      uint32_t q[4];
+      if (C::kQShared) {
+        const uint4 x = sq[k * 32 + lane];
+        q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
+      } else {
+        q[0] = qf[k][0], q[1] = qf[k][1], q[2] = qf[k][2], q[3] = qf[k][3];
+      }
 #pragma unroll
       for (int i = 0; i < KS / 16; ++i) {
         uint32_t kb[4];
         ldsm4(sk + swz<DP>(i * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + ((lane >> 3) & 1)), kb);
-        mma16816(sc[2 * i], qf[k], kb[0], kb[1]);
-        mma16816(sc[2 * i + 1], qf[k], kb[2], kb[3]);
+        mma16816(sc[2 * i], q, kb[0], kb[1]);
+        mma16816(sc[2 * i + 1], q, kb[2], kb[3]);
       }
-    float mx[2] = {-INFINITY, -INFINITY};
+    }
+    if (j + KS > least) {   // keys that some row does not see
+#pragma unroll
+      for (int i = 0; i < KS / 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (j + i * 8 + (lane & 3) * 2 + (k & 1) >= min(j1, seen[k >> 1])) sc[i][k] = -INFINITY;
+    }
+    float mx[2] = {-INFINITY, -INFINITY}, base[2];
 #pragma unroll
     for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int at = j + i * 8 + (lane & 3) * 2 + (k & 1);
-        sc[i][k] = at < min(j1, seen[k >> 1]) ? sc[i][k] * p.scale_log2 : -INFINITY;
-        mx[k >> 1] = fmaxf(mx[k >> 1], sc[i][k]);
-      }
-    float base[2], a[2];
+      for (int k = 0; k < 4; ++k) mx[k >> 1] = fmaxf(mx[k >> 1], sc[i][k]);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      const float mn = fmaxf(m[h], mx[h]);
-      base[h] = mn == -INFINITY ? 0.f : mn;      // a row without keys so far: every 2^(s - base) is 0
-      a[h] = exp2f(m[h] - base[h]);
-      m[h] = mn;
-      l[h] *= a[h];
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * p.scale_log2;
+    }
+    if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
+      float a[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float mn = fmaxf(m[h], mx[h]);
+        a[h] = mn == -INFINITY ? 1.f : exp2f(m[h] - mn);
+        m[h] = mn;
+        l[h] *= a[h];
+      }
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[i][k] *= a[k >> 1];
     }
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[i][k] *= a[k >> 1];
+    for (int h = 0; h < 2; ++h) base[h] = m[h] == -INFINITY ? 0.f : m[h];   // a row without keys so far: every 2^(s - base) is 0
 #pragma unroll
     for (int i = 0; i < KS / 16; ++i) {
       uint32_t pf[4];
@@ -237,7 +275,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
       for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float e0 = exp2f(sc[2 * i + c][2 * h] - base[h]), e1 = exp2f(sc[2 * i + c][2 * h + 1] - base[h]);
+          const float e0 = attn_tc::ex2(fmaf(sc[2 * i + c][2 * h], p.scale_log2, -base[h])),
+                      e1 = attn_tc::ex2(fmaf(sc[2 * i + c][2 * h + 1], p.scale_log2, -base[h]));
           l[h] += e0 + e1;
           pf[h + 2 * c] = tc::pack2_bf16(e0, e1);
         }
@@ -259,8 +298,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
   // the warps' results joined through shared memory, where the rings were
   cp_wait<0>();
   __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(rows_smem_dyn);            // [warp][16][DP]
-  float2* sm_ml = reinterpret_cast<float2*>(sm_o + kRowWarps * kRowTile * DP);   // [warp][16]
+  float* sm_o = reinterpret_cast<float*>(rows_smem_dyn + C::kQ);          // [warp][16][DP]
+  float2* sm_ml = reinterpret_cast<float2*>(sm_o + W * kRowTile * DP);   // [warp][16]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = lane / 4 + 8 * h;
@@ -277,10 +316,10 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) paged_rows_kernel(const Att
     const int rl = i / quads, d = i % quads * 4, r = r0 + rl;
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) top = fmaxf(top, sm_ml[w * kRowTile + rl].x);
+    for (int w = 0; w < W; ++w) top = fmaxf(top, sm_ml[w * kRowTile + rl].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kRowWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float2 ml = sm_ml[w * kRowTile + rl];
       const float c = ml.y == 0.f ? 0.f : exp2f(ml.x - top);
       const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * kRowTile + rl) * DP + d);
@@ -315,8 +354,8 @@ static bool rows_eligible(const Attn& p) {
          p.q_t % 2 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && p.o_t % 4 == 0;
 }
 
-template <int DP>
-static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+template <int DP, int W>
+static int launch_rows_w(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
   static bool done[64] = {false};
   static std::mutex mu;
   int dev = 0;
@@ -324,7 +363,8 @@ static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int d
   {
     std::lock_guard<std::mutex> g(mu);
     if (dev >= 0 && dev < 64 && !done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem(DP));
+      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<DP, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           Rows<DP, W>::kSmem);
       if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       done[dev] = true;
     }
@@ -333,9 +373,16 @@ static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int d
   const int64_t blocks = (rows + kRowTile - 1) / kRowTile;
   const int64_t grid = blocks * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
-  launch_pdl(paged_rows_kernel<DP>, dim3((unsigned)grid), dim3(kRowWarps * 32), rows_smem(DP), st, p, phase, splits,
+  launch_pdl(paged_rows_kernel<DP, W>, dim3((unsigned)grid), dim3(W * 32), Rows<DP, W>::kSmem, st, p, phase, splits,
              (int)blocks, slot0, direct, early);
   return launch_status("paged_rows");
+}
+
+template <int DP>
+static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+  static const char* e = getenv("ROWS_W");
+  return e && *e == '2' ? launch_rows_w<DP, 2>(p, phase, splits, slot0, direct, early, st)
+                        : launch_rows_w<DP, 4>(p, phase, splits, slot0, direct, early, st);
 }
 
 static int launch_rows(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {

@@ -6,7 +6,6 @@ sibling modules (``cutile_gelu`` …) allocate their outputs and delegate here.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -25,14 +24,6 @@ def _row_stride(t: torch.Tensor, what: str) -> int:
         raise ValueError(f"{what}: expected a 2-D tensor with contiguous rows, got shape "
                          f"{tuple(t.shape)} strides {t.stride()}")
     return t.stride(0) if t.size(0) > 1 else max(t.size(1), t.stride(0))
-
-
-_HERE = contextlib.nullcontext()
-
-
-def kv_device(kv):
-    """Context in which the device of `kv` is the current one (a launch goes to the current device)."""
-    return _HERE if kv.device.index == torch.cuda.current_device() else torch.cuda.device(kv.device)
 
 
 def embedding(idx: torch.Tensor, weight: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
@@ -213,34 +204,45 @@ def _strides3(t: torch.Tensor | None):
     return None if t is None else L.strides3(*t.stride()[:3])
 
 
+def _on_device(kv, fn, *args) -> int:
+    """fn(*args, stream) with the device of `kv` current (a launch goes to the current device)."""
+    index = kv.device.index
+    if index == torch.cuda.current_device():
+        return fn(*args, L.stream_ptr(kv.device))
+    with torch.cuda.device(index):
+        return fn(*args, L.stream_ptr(kv.device))
+
+
 def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: torch.Tensor | None, kv,
                     cos_sin: torch.Tensor | None = None, interleaved: bool = False) -> None:
     """k, v [B, K, T, D] views into the pages of `kv` (a PagedKV); with cos_sin [n_pos, rot] the keys
     and q [B, H, T, D] are rotated, q into q_out."""
     n_pos, rot = cos_sin.shape if cos_sin is not None else (0, 0)
     heads = q.shape[1] if q is not None else kv.n_kv_head
-    with kv_device(kv):
-        L.check(L.lib().gpt_paged_kv_append(_ptr(q), _strides3(q), k.data_ptr(), _strides3(k), v.data_ptr(), _strides3(v),
-                                            _ptr(q_out), _strides3(q_out), k.shape[2], heads, kv._ref, _ptr(cos_sin),
-                                            n_pos, rot, int(interleaved), kv._dtype_code, L.stream_ptr()),
-                "gpt_paged_kv_append")
+    status = _on_device(kv, L.lib().gpt_paged_kv_append, _ptr(q), _strides3(q), k.data_ptr(), _strides3(k), v.data_ptr(),
+                        _strides3(v), _ptr(q_out), _strides3(q_out), k.shape[2], heads, kv._ref, _ptr(cos_sin), n_pos, rot,
+                        int(interleaved), kv._dtype_code)
+    if status:
+        L.check(status, "gpt_paged_kv_append")
 
 
 def shared_prefix_attention(q: torch.Tensor, kv, out: torch.Tensor, scale: float,
                             workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q, out [B, H, T, D] views over the cache `kv` (a PagedKV). The workspace, kv.workspace_bytes(H, T)
     bytes of uint8, is allocated (on the current stream) when it is None."""
-    H, T = q.shape[1], q.shape[2]
-    need = kv.workspace_bytes(H, T)
+    _, H, T, _ = q.shape
     if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    elif workspace.device != q.device or not workspace.is_contiguous():
+        have = kv.workspace_bytes(H, T)
+        if have:
+            workspace = torch.empty(have, dtype=torch.uint8, device=kv.device)
+    elif workspace.device != kv.device or not workspace.is_contiguous():
         raise ValueError("shared_prefix_attention: the workspace must be a contiguous tensor on the cache's device")
-    have = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    with kv_device(kv):
-        L.check(L.lib().gpt_attention_shared_prefix(q.data_ptr(), _strides3(q), out.data_ptr(), _strides3(out), T, H,
-                                                    kv._ref, float(scale), _ptr(workspace), have, kv._dtype_code,
-                                                    L.stream_ptr()), "gpt_attention_shared_prefix")
+    else:
+        have = workspace.numel() * workspace.element_size()
+    status = _on_device(kv, L.lib().gpt_attention_shared_prefix, q.data_ptr(), _strides3(q), out.data_ptr(), _strides3(out),
+                        T, H, kv._ref, scale, _ptr(workspace), have, kv._dtype_code)
+    if status:
+        L.check(status, "gpt_attention_shared_prefix")
     return out
 
 

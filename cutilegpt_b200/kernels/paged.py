@@ -116,7 +116,8 @@ class PagedKV:
 
 def _rows(t, name: str, kv: PagedKV, heads: int | None, tokens: int | None) -> torch.Tensor:
     """A (batch, heads, tokens, head_dim) tensor of the cache's type and device, head_dim contiguous."""
-    t = as_cuda(t, name)
+    if not isinstance(t, torch.Tensor):
+        t = as_cuda(t, name)
     shape = t.shape
     if (len(shape) != 4 or shape[0] != kv.batch or shape[3] != kv.head_dim or (heads is not None and shape[1] != heads)
             or (tokens is not None and shape[2] != tokens)):
@@ -152,7 +153,7 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
         raise ValueError(f"cos_sin: expected a contiguous float32 [n_pos, rot] table with even rot <= {kv.head_dim} on "
                          f"{kv.device}, got {cos_sin.dtype} {tuple(cos_sin.shape)} on {cos_sin.device}")
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         if _rows(q_out, "q_out", kv, q.shape[1], tokens) is not q_out:
             raise ValueError("q_out: head_dim must be contiguous")
@@ -175,7 +176,7 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
     if heads == 0 or heads % kv.n_kv_head:
         raise ValueError(f"shared_prefix_attention: {heads} heads are no multiple of {kv.n_kv_head} key heads")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif _rows(out, "out", kv, heads, tokens) is not out:
         raise ValueError("out: head_dim must be contiguous")
     return ops.shared_prefix_attention(q, kv, out, 1.0 / math.sqrt(kv.head_dim) if scale is None else scale, workspace)
