@@ -117,8 +117,8 @@ static int launch(Kernel kernel, const Attn& p, int phase, int splits, int two, 
       a.early = early;
       return launch_tc(p, a, st);
     }
-    if (kernel == kRows) return launch_rows(p, phase, splits, slot0, direct, early, st);
   }
+  if (kernel == kRows) return launch_rows<T>(p, phase, splits, slot0, direct, early, st);
   return launch_simt<T>(p, phase, splits, slot0, direct, st);
 }
 
@@ -217,7 +217,7 @@ int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H, const g
     return 0;
   // the largest over the kernels that the alignment of q and out may ask for
   int64_t most = 0;
-  for (int k = gpt::paged::kSimt; k <= (dtype == GPT_BF16 ? gpt::paged::kTc : gpt::paged::kSimt); ++k) {
+  for (int k = gpt::paged::kSimt; k <= (dtype == GPT_BF16 ? gpt::paged::kTc : gpt::paged::kRows); ++k) {
     const int64_t n = gpt::paged::make_plan(T, H, kv, (gpt::paged::Kernel)k).bytes;
     most = n > most ? n : most;
   }
@@ -275,10 +275,9 @@ int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* o
   p.share = (int)(H / kv->kv_heads);
   p.D = (int)kv->head_dim;
   p.scale_log2 = scale * gpt::paged::kLog2e;
-  const gpt::paged::Kernel best = dtype != GPT_BF16              ? gpt::paged::kSimt
-                                  : gpt::paged::tc_eligible(p)   ? gpt::paged::kTc
-                                  : gpt::paged::rows_eligible(p) ? gpt::paged::kRows
-                                                                 : gpt::paged::kSimt;
+  const gpt::paged::Kernel best = dtype == GPT_BF16 && gpt::paged::tc_eligible(p)              ? gpt::paged::kTc
+                                  : gpt::paged::rows_eligible(p, dtype == GPT_BF16 ? 2 : 4) ? gpt::paged::kRows
+                                                                                            : gpt::paged::kSimt;
   const gpt::paged::Plan pl = gpt::paged::make_plan(T, H, kv, best);
   GPT_CHECK_ARG(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes),
                 "%s: workspace of %lld bytes required", what, (long long)pl.bytes);

@@ -1,19 +1,22 @@
-// Attention over the paged cache for few rows a key head (bf16): one decode
-// step, or the few tokens of a draft.
+// Attention over the paged cache for few rows a key head: one decode step, or
+// the few tokens of a draft.
 //
 // Every key and value is read once and meets at most 16 rows, so the kernel is
-// bound by HBM: 4 D bytes a key against 64 D multiply-adds. A CTA takes 16 rows
+// bound by HBM: 2 D e bytes a key against 32 D multiply-adds. A CTA takes 16 rows
 // of one key head (phases as in paged.cuh) and one of `splits` equal shares of
-// the phase's keys. Its four warps work alone until the end: warp w takes the
-// steps of KS keys w, w + 4, ... of the share, copies them by cp.async
+// the phase's keys. Its W warps work alone until the end: warp w takes the
+// steps of KS keys w, w + W, ... of the share, copies them by cp.async
 // (16 bytes a lane, addresses from the page table, zeros behind the length) into its
-// own ring of kRing steps, and keeps running maxima, sums and the 16 x D
-// accumulator in registers: S = Q Kᵀ and O += P V are m16n8k16 tensor-core
-// products (16 rows cannot fill the 128 rows of a tcgen05 tile; those run in
-// paged_tc.cu). No barrier stands between a warp's loads and its products, so a
-// CTA keeps 4 x (kRing - 1) steps of 8 KB in flight, two CTAs of an SM 128 KB.
-// P is rounded to bf16 for the product with V (as the V it meets); its sum is
-// taken before the rounding, in fp32.
+// own ring, and keeps running maxima, sums and the 16 x D accumulator in
+// registers. S = Q Kᵀ and O += P V are tensor-core products of 16 rows
+// (mma.sync: 16 rows cannot fill the 128 rows of a tcgen05 tile; those run in paged_tc.cu).
+// No barrier stands between a warp's loads and its products; 12 to 16 warps of an
+// SM keep 96 to 128 KB in flight.
+//
+// bf16: m16n8k16. P is rounded to bf16 for its product with V, its sum is taken before.
+// fp32: m16n8k8 on TF32 parts. A value x is hi + lo, hi = x to 11 bits, lo = (x - hi) to
+// 11 bits: x is met to 2^-22, and hi hi + hi lo + lo hi leaves out 2^-22 of a product. The order of a
+// contraction is free, so a lane's operands are those that one 16-byte read gives it.
 #include "paged.cuh"
 
 namespace gpt {
@@ -21,26 +24,33 @@ namespace paged {
 
 constexpr int kRowTile = 16;
 
-template <int DP, int W>   // W warps
+template <typename T, int DP, int W>   // DP: head size padded to a power of two
 struct Rows {
-  static constexpr int kKeys = DP >= 64 ? 16 : 1024 / DP;      // keys of a warp's step
-  static constexpr int kTile = kKeys * DP * 2;                 // bytes of a step's keys
-  static constexpr int kRing = DP == 128 ? 2 : 3;              // steps of a warp's ring
-  static constexpr int kCtas = (DP == 128 ? 12 : 16) / W;      // of an SM
-  static constexpr bool kQShared = DP == 128;                  // Q fragments are read from shared memory at every step
+  static constexpr bool kWide = sizeof(T) == 4;
+  static constexpr int kKeys = kWide ? (DP == 128 ? 8 : DP == 64 ? 16 : 32) : (DP >= 64 ? 16 : 1024 / DP);   // of a warp's step
+  static constexpr int kTile = kKeys * DP * (int)sizeof(T);    // bytes of a step's keys
+  static constexpr int kRing = kTile > 2048 ? 2 : 3;           // steps of a warp's ring
+  static constexpr int kCtas = (kWide ? 8 : DP == 128 ? 12 : 16) / W;   // of an SM
+  // Q fragments in shared memory, read at every step, where they would take too many registers
+  static constexpr bool kQShared = kWide || DP == 128;
+  static constexpr int kQSteps = kWide ? DP / 4 : DP / 16;     // uint4 of a lane
+  static constexpr int kQ = kQShared ? kQSteps * 512 : 0;
   static constexpr int kRings = W * kRing * 2 * kTile;
   static constexpr int kMerge = W * kRowTile * (DP + 2) * 4;
-  static constexpr int kQ = kQShared ? kRowTile * DP * 2 : 0;
   static constexpr int kSmem = (kRings > kMerge ? kRings : kMerge) + kQ;
 };
 
-// Byte offset of 16-byte chunk c of row r in a tile of rows of DP bf16, chunks permuted
-// inside a row so that eight consecutive rows of one chunk column hit eight bank groups.
-template <int DP>
+// Byte offset of 16-byte chunk c of row r in a tile of rows of DP values, chunks permuted
+// inside a row so that the chunks that one read touches lie in different bank groups.
+template <typename T, int DP>
 __device__ __forceinline__ uint32_t swz(int r, int c) {
-  constexpr int kChunks = DP / 8;
-  const int x = kChunks >= 8 ? (r & 7) : kChunks == 4 ? ((r >> 1) & 3) : ((r >> 2) & 1);
-  return (uint32_t)(r * DP * 2 + ((c ^ x) << 4));
+  constexpr int kChunks = DP * (int)sizeof(T) / 16;
+  int x;
+  if (sizeof(T) == 4)   // reads of rows 0..7 by 4 chunks, and of rows 0, 2, 4, 6 by 8 floats
+    x = (((r ^ (r >> 1)) & 1) << 2) | (((r >> 2) & 1) << 1) | ((r >> 1) & 1);
+  else                  // reads of 8 rows of one chunk column
+    x = kChunks >= 8 ? (r & 7) : kChunks == 4 ? ((r >> 1) & 3) : ((r >> 2) & 1);
+  return (uint32_t)(r * DP * (int)sizeof(T) + ((c ^ x) << 4));
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
@@ -62,11 +72,41 @@ __device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
+__device__ __forceinline__ void lds128(uint32_t addr, float (&r)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3])
+               : "r"(addr)
+               : "memory");
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma1688(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = to_tf32(x);
+  lo = to_tf32(x - __uint_as_float(hi));
+}
+// c += a b in three TF32 products, the small ones first.
+__device__ __forceinline__ void mma_split(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
+  uint32_t h0, l0, h1, l1;
+  split_tf32(b0, h0, l0);
+  split_tf32(b1, h1, l1);
+  mma1688(c, al, h0, h1);
+  mma1688(c, ah, l0, l1);
+  mma1688(c, ah, h0, h1);
 }
 
 // One row's four columns joined with the partial slots first .. first + n - 1, eight at a time.
@@ -102,13 +142,22 @@ __device__ __forceinline__ void join4(const Attn& p, int first, int n, int64_t r
     }
   }
 }
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, float4 v) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(dst) = v;
+  else
+    *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack2_bf16(v.x, v.y), tc::pack2_bf16(v.z, v.w));
+}
 
-template <int DP, int W>
-__global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kernel(const Attn p, int phase, int splits,
-                                                                                  int blocks, int slot0, int direct,
-                                                                                  int early) {
-  using C = Rows<DP, W>;
-  constexpr int KS = C::kKeys, kChunks = DP / 8, kLoads = KS * kChunks / 32, kTile = C::kTile, kRing = C::kRing;
+template <typename T, int DP, int W>
+__global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_kernel(const Attn p, int phase, int splits,
+                                                                                     int blocks, int slot0, int direct,
+                                                                                     int early) {
+  using C = Rows<T, DP, W>;
+  constexpr bool kWide = C::kWide;
+  constexpr int KS = C::kKeys, kPer = 16 / (int)sizeof(T), kChunks = DP / kPer, kLoads = KS * kChunks / 32;
+  constexpr int kTile = C::kTile, kRing = C::kRing;
   extern __shared__ __align__(128) uint8_t rows_smem_dyn[];
   // With `early` the launch before is this call's prefix launch, whose every CTA has waited for all
   // that came before it: what is read and written here is then safe, but for the prefix's partial results.
@@ -124,34 +173,28 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
   const int rs = p.T * p.share;                       // rows of a sequence
   const int rows = rs * (phase == kPrefix ? p.per : 1);
   const int r0 = block * kRowTile;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
   const Keys keys(p, phase, who);
   const int n = keys.n();
   const int chunk = ((n + splits - 1) / splits + KS - 1) / KS * KS;
   const int j0 = min(n, split * chunk);
   int j1 = min(n, j0 + chunk);
 
-  // Q in the A fragments: rows lane / 4 and lane / 4 + 8
-  uint32_t qf[DP / 16][4];
+  // rows lane / 4 and lane / 4 + 8 of the tile
+  const T* src[2];
+  bool live[2];
   int seen[2];                      // keys below this one are the row's
   int most = 0, least = n;          // the largest and the smallest of the tile's
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const int r = r0 + lane / 4 + 8 * half;
-    const bool live = r < rows;
-    const int b = b0 + (live ? r / rs : 0), rr = live ? r % rs : 0, t = rr / p.share;
-    seen[half] = !live ? 0 : phase == kPrefix ? n : max(0, keys.n_pre + keys.n_own - p.T + t + 1);
-    if (live && phase != kPrefix && keys.n_own - p.T + t < 0) seen[half] = 0;   // padding sees nothing
-    most = max(most, seen[half]);
-    if (live) least = min(least, seen[half]);
-    const __nv_bfloat16* src = (const __nv_bfloat16*)p.q + b * p.q_b + (int64_t)(kh * p.share + rr % p.share) * p.q_h + t * p.q_t;
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int d = k * 16 + c * 8 + (lane & 3) * 2;
-        qf[k][half + 2 * c] = live && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
-      }
+  for (int h = 0; h < 2; ++h) {
+    const int r = r0 + lane / 4 + 8 * h;
+    live[h] = r < rows;
+    const int b = b0 + (live[h] ? r / rs : 0), rr = live[h] ? r % rs : 0, t = rr / p.share;
+    const int last = keys.n_own - p.T + t;            // own key; below 0 the row is padding and sees nothing
+    seen[h] = !live[h] ? 0 : phase == kPrefix ? n : last < 0 ? 0 : keys.n_pre + last + 1;
+    most = max(most, seen[h]);
+    if (live[h]) least = min(least, seen[h]);
+    src[h] = (const T*)p.q + b * p.q_b + (int64_t)(kh * p.share + rr % p.share) * p.q_h + t * p.q_t;
   }
   j1 = min(j1, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
   least = min(j1, (int)__reduce_min_sync(0xffffffffu, (unsigned)least));
@@ -159,14 +202,6 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rows_smem_dyn) + C::kQ + warp * (kRing * 2 * kTile);
   if (p.D < DP) {   // columns behind D stay zeros
     for (int i = threadIdx.x; i < C::kRings / 16; i += blockDim.x) reinterpret_cast<uint4*>(rows_smem_dyn + C::kQ)[i] = uint4{};
-    __syncthreads();
-  }
-  uint4* sq = reinterpret_cast<uint4*>(rows_smem_dyn);   // with kQShared: the fragments, [k][lane]
-  if (C::kQShared) {
-    if (warp == 0) {
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) sq[k * 32 + lane] = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
-    }
     __syncthreads();
   }
   const int steps = j1 > j0 + warp * KS ? (j1 - j0 - warp * KS + W * KS - 1) / (W * KS) : 0;
@@ -187,13 +222,54 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
     for (int i = 0; i < kLoads; ++i) {
       const int r = i * (32 / kChunks) + lane / kChunks;
       const int64_t o = __shfl_sync(0xffffffffu, off[i * (32 / kChunks) / 32], r & 31);
-      if (c * 8 < p.D) {
-        const int64_t at = (o < 0 ? 0 : o) + c * 8;
-        cp_async16(dst + swz<DP>(r, c), (const __nv_bfloat16*)p.k + at, o >= 0);
-        cp_async16(dst + kTile + swz<DP>(r, c), (const __nv_bfloat16*)p.v + at, o >= 0);
+      if (c * kPer < p.D) {
+        const int64_t at = (o < 0 ? 0 : o) + c * kPer;
+        cp_async16(dst + swz<T, DP>(r, c), (const T*)p.k + at, o >= 0);
+        cp_async16(dst + kTile + swz<T, DP>(r, c), (const T*)p.v + at, o >= 0);
       }
     }
     cp_commit();
+  };
+  for (int s = 0; s < kRing - 1; ++s) {
+    locate(s);
+    fetch(s);
+  }
+  locate(kRing - 1);
+
+  // Q in the A fragments, with kQShared in shared memory as [step][lane]
+  uint4* sq = reinterpret_cast<uint4*>(rows_smem_dyn);
+  uint4 qf[C::kQShared ? 1 : C::kQSteps];
+  if constexpr (kWide) {
+    for (int k = warp; k < DP / 8; k += W) {
+      // the contraction step's elements of this lane: 16 (k / 2) + 4 quad + 2 (k % 2) and the next one
+      const int d = 16 * (k / 2) + 4 * quad + 2 * (k % 2);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) split_tf32(live[i & 1] && d + (i >> 1) < p.D ? src[i & 1][d + (i >> 1)] : 0.f, hi[i], lo[i]);
+      sq[2 * k * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      sq[(2 * k + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      if (C::kQShared && k % W != warp) continue;
+      uint32_t a[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = k * 16 + (i >> 1) * 8 + quad * 2;
+        a[i] = live[i & 1] && d < p.D ? *reinterpret_cast<const uint32_t*>(src[i & 1] + d) : 0u;
+      }
+      const uint4 x = make_uint4(a[0], a[1], a[2], a[3]);
+      if (C::kQShared)
+        sq[k * 32 + lane] = x;
+      else
+        qf[k] = x;
+    }
+  }
+  if (C::kQShared) __syncthreads();
+  auto q_frag = [&](int k, uint32_t (&a)[4]) {
+    const uint4 x = C::kQShared ? sq[k * 32 + lane] : qf[C::kQShared ? 0 : k];
+    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
   };
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DP / 8][4];
@@ -201,11 +277,6 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
   for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
-  for (int s = 0; s < kRing - 1; ++s) {
-    locate(s);
-    fetch(s);
-  }
-  locate(kRing - 1);
   for (int s = 0; s < steps; ++s) {
     cp_wait<kRing - 2>();
     __syncwarp();
@@ -218,21 +289,35 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
     for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) sc[i][k] = 0.f;
+    if constexpr (kWide) {
 #pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      uint32_t q[4];
-      if (C::kQShared) {
-        const uint4 x = sq[k * 32 + lane];
-        q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
-      } else {
-        q[0] = qf[k][0], q[1] = qf[k][1], q[2] = qf[k][2], q[3] = qf[k][3];
+      for (int k = 0; k < DP / 16; ++k) {
+        uint32_t ah[2][4], al[2][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          q_frag(4 * k + 2 * u, ah[u]);
+          q_frag(4 * k + 2 * u + 1, al[u]);
+        }
+#pragma unroll
+        for (int i = 0; i < KS / 8; ++i) {
+          float kv[4];
+          lds128(sk + swz<T, DP>(i * 8 + lane / 4, k * 4 + quad), kv);
+          mma_split(sc[i], ah[0], al[0], kv[0], kv[1]);
+          mma_split(sc[i], ah[1], al[1], kv[2], kv[3]);
+        }
       }
+    } else {
 #pragma unroll
-      for (int i = 0; i < KS / 16; ++i) {
-        uint32_t kb[4];
-        ldsm4(sk + swz<DP>(i * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + ((lane >> 3) & 1)), kb);
-        mma16816(sc[2 * i], q, kb[0], kb[1]);
-        mma16816(sc[2 * i + 1], q, kb[2], kb[3]);
+      for (int k = 0; k < DP / 16; ++k) {
+        uint32_t a[4];
+        q_frag(k, a);
+#pragma unroll
+        for (int i = 0; i < KS / 16; ++i) {
+          uint32_t kb[4];
+          ldsm4(sk + swz<T, DP>(i * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + ((lane >> 3) & 1)), kb);
+          mma16816(sc[2 * i], a, kb[0], kb[1]);
+          mma16816(sc[2 * i + 1], a, kb[2], kb[3]);
+        }
       }
     }
     if (j + KS > least) {   // keys that some row does not see
@@ -240,7 +325,7 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
       for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (j + i * 8 + (lane & 3) * 2 + (k & 1) >= min(j1, seen[k >> 1])) sc[i][k] = -INFINITY;
+          if (j + i * 8 + quad * 2 + (k & 1) >= min(j1, seen[k >> 1])) sc[i][k] = -INFINITY;
     }
     float mx[2] = {-INFINITY, -INFINITY}, base[2];
 #pragma unroll
@@ -269,23 +354,44 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
 #pragma unroll
     for (int h = 0; h < 2; ++h) base[h] = m[h] == -INFINITY ? 0.f : m[h];   // a row without keys so far: every 2^(s - base) is 0
 #pragma unroll
-    for (int i = 0; i < KS / 16; ++i) {
-      uint32_t pf[4];
+    for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int k = 0; k < 4; ++k) {
+        sc[i][k] = attn_tc::ex2(fmaf(sc[i][k], p.scale_log2, -base[k >> 1]));
+        l[k >> 1] += sc[i][k];
+      }
+    if constexpr (kWide) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float e0 = attn_tc::ex2(fmaf(sc[2 * i + c][2 * h], p.scale_log2, -base[h])),
-                      e1 = attn_tc::ex2(fmaf(sc[2 * i + c][2 * h + 1], p.scale_log2, -base[h]));
-          l[h] += e0 + e1;
-          pf[h + 2 * c] = tc::pack2_bf16(e0, e1);
+      for (int i = 0; i < KS / 8; ++i) {   // contraction index quad is key 2 quad, quad + 4 is key 2 quad + 1
+        uint32_t ah[4], al[4];
+        split_tf32(sc[i][0], ah[0], al[0]);
+        split_tf32(sc[i][2], ah[1], al[1]);
+        split_tf32(sc[i][1], ah[2], al[2]);
+        split_tf32(sc[i][3], ah[3], al[3]);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {   // column index g of product u is element 32 d + 4 g + u
+          float v0[4], v1[4];
+          lds128(sv + swz<T, DP>(i * 8 + 2 * quad, d * 8 + lane / 4), v0);
+          lds128(sv + swz<T, DP>(i * 8 + 2 * quad + 1, d * 8 + lane / 4), v1);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) mma_split(o[4 * d + u], ah, al, v0[u], v1[u]);
         }
+      }
+    } else {
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) {
-        uint32_t vb[4];
-        ldsm4_t(sv + swz<DP>(i * 16 + (lane & 15), d * 2 + (lane >> 4)), vb);
-        mma16816(o[2 * d], pf, vb[0], vb[1]);
-        mma16816(o[2 * d + 1], pf, vb[2], vb[3]);
+      for (int i = 0; i < KS / 16; ++i) {
+        uint32_t pf[4];
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) pf[h + 2 * c] = tc::pack2_bf16(sc[2 * i + c][2 * h], sc[2 * i + c][2 * h + 1]);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+          uint32_t vb[4];
+          ldsm4_t(sv + swz<T, DP>(i * 16 + (lane & 15), d * 2 + (lane >> 4)), vb);
+          mma16816(o[2 * d], pf, vb[0], vb[1]);
+          mma16816(o[2 * d + 1], pf, vb[2], vb[3]);
+        }
       }
     }
   }
@@ -298,21 +404,30 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
   // the warps' results joined through shared memory, where the rings were
   cp_wait<0>();
   __syncthreads();
-  float* sm_o = reinterpret_cast<float*>(rows_smem_dyn + C::kQ);          // [warp][16][DP]
+  float* sm_o = reinterpret_cast<float*>(rows_smem_dyn + C::kQ);         // [warp][16][DP]
   float2* sm_ml = reinterpret_cast<float2*>(sm_o + W * kRowTile * DP);   // [warp][16]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = lane / 4 + 8 * h;
-    if ((lane & 3) == 0) sm_ml[warp * kRowTile + r] = make_float2(m[h], l[h]);
+    if (quad == 0) sm_ml[warp * kRowTile + r] = make_float2(m[h], l[h]);
+    float* dst = sm_o + (warp * kRowTile + r) * DP;
+    if constexpr (kWide) {
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i)
-      *reinterpret_cast<float2*>(sm_o + (warp * kRowTile + r) * DP + i * 8 + (lane & 3) * 2) =
-          make_float2(o[i][2 * h], o[i][2 * h + 1]);
+      for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          *reinterpret_cast<float4*>(dst + 32 * d + 4 * (2 * quad + e)) =
+              make_float4(o[4 * d][2 * h + e], o[4 * d + 1][2 * h + e], o[4 * d + 2][2 * h + e], o[4 * d + 3][2 * h + e]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+        *reinterpret_cast<float2*>(dst + i * 8 + quad * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+    }
   }
   __syncthreads();
   if (early) pdl_wait();   // the prefix launch's partial results; its end, for whatever comes after this launch
-  const int live = min(kRowTile, rows - r0), quads = p.D / 4;
-  for (int i = threadIdx.x; i < live * quads; i += blockDim.x) {
+  const int n_live = min(kRowTile, rows - r0), quads = p.D / 4;
+  for (int i = threadIdx.x; i < n_live * quads; i += blockDim.x) {
     const int rl = i / quads, d = i % quads * 4, r = r0 + rl;
     float top = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -335,10 +450,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
       const bool padding = keys.n_own - p.T + t < 0;
       if (!padding && p.n_pre > 0) join4(p, 0, p.n_pre, row, d, top, sum, acc);
       const float inv = padding ? 0.f : 1.f / sum;
-      uint2 w;
-      w.x = padding ? 0u : tc::pack2_bf16(acc.x * inv, acc.y * inv);
-      w.y = padding ? 0u : tc::pack2_bf16(acc.z * inv, acc.w * inv);
-      *reinterpret_cast<uint2*>((__nv_bfloat16*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d) = w;
+      store4((T*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d,
+             padding ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     } else {
       const int64_t at = (int64_t)(slot0 + split) * p.B * p.T * p.H + row;
       if (d == 0) p.ml[at] = make_float2(top, sum);
@@ -347,15 +460,22 @@ __global__ void __launch_bounds__(W * 32, (Rows<DP, W>::kCtas)) paged_rows_kerne
   }
 }
 
-// Whether the kernel serves the call: 16-byte rows of keys and values, 4-byte pairs of q, 8-byte quads of out.
-static bool rows_eligible(const Attn& p) {
-  if (p.D % 8 || p.D > 128 || !aligned(p.k, 16) || !aligned(p.v, 16) || !aligned(p.q, 4) || !aligned(p.out, 8)) return false;
-  return p.page_stride % 8 == 0 && p.head_stride % 8 == 0 && p.slot_stride % 8 == 0 && p.q_b % 2 == 0 && p.q_h % 2 == 0 &&
-         p.q_t % 2 == 0 && p.o_b % 4 == 0 && p.o_h % 4 == 0 && p.o_t % 4 == 0;
+// Whether the kernel serves the call: 16-byte rows of keys and values, pairs of q for bf16, quads of out.
+static bool rows_eligible(const Attn& p, int size) {
+  const int per = 16 / size;
+  if (p.D % per || p.D > 128 || !aligned(p.k, 16) || !aligned(p.v, 16) || !aligned(p.q, 4) || !aligned(p.out, 4 * size)) return false;
+  for (int64_t s : {p.page_stride, p.head_stride, p.slot_stride})
+    if (s % per) return false;
+  for (int64_t s : {p.q_b, p.q_h, p.q_t})
+    if (s % (size == 2 ? 2 : 1)) return false;
+  for (int64_t s : {p.o_b, p.o_h, p.o_t})
+    if (s % 4) return false;
+  return true;
 }
 
-template <int DP, int W>
+template <typename T, int DP, int W>
 static int launch_rows_w(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+  using C = Rows<T, DP, W>;
   static bool done[64] = {false};
   static std::mutex mu;
   int dev = 0;
@@ -363,8 +483,7 @@ static int launch_rows_w(const Attn& p, int phase, int splits, int slot0, int di
   {
     std::lock_guard<std::mutex> g(mu);
     if (dev >= 0 && dev < 64 && !done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<DP, W>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           Rows<DP, W>::kSmem);
+      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, DP, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       done[dev] = true;
     }
@@ -373,23 +492,25 @@ static int launch_rows_w(const Attn& p, int phase, int splits, int slot0, int di
   const int64_t blocks = (rows + kRowTile - 1) / kRowTile;
   const int64_t grid = blocks * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
-  launch_pdl(paged_rows_kernel<DP, W>, dim3((unsigned)grid), dim3(W * 32), Rows<DP, W>::kSmem, st, p, phase, splits,
-             (int)blocks, slot0, direct, early);
+  launch_pdl(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, phase, splits, (int)blocks,
+             slot0, direct, early);
   return launch_status("paged_rows");
 }
 
-template <int DP>
+template <typename T, int DP>
 static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
   static const char* e = getenv("ROWS_W");
-  return e && *e == '2' ? launch_rows_w<DP, 2>(p, phase, splits, slot0, direct, early, st)
-                        : launch_rows_w<DP, 4>(p, phase, splits, slot0, direct, early, st);
+  return e && *e == '2' ? launch_rows_w<T, DP, 2>(p, phase, splits, slot0, direct, early, st)
+                        : launch_rows_w<T, DP, 4>(p, phase, splits, slot0, direct, early, st);
 }
 
+template <typename T>
 static int launch_rows(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
-  if (p.D <= 16) return launch_rows_dp<16>(p, phase, splits, slot0, direct, early, st);
-  if (p.D <= 32) return launch_rows_dp<32>(p, phase, splits, slot0, direct, early, st);
-  if (p.D <= 64) return launch_rows_dp<64>(p, phase, splits, slot0, direct, early, st);
-  return launch_rows_dp<128>(p, phase, splits, slot0, direct, early, st);
+  if constexpr (sizeof(T) == 2)
+    if (p.D <= 16) return launch_rows_dp<T, 16>(p, phase, splits, slot0, direct, early, st);
+  if (p.D <= 32) return launch_rows_dp<T, 32>(p, phase, splits, slot0, direct, early, st);
+  if (p.D <= 64) return launch_rows_dp<T, 64>(p, phase, splits, slot0, direct, early, st);
+  return launch_rows_dp<T, 128>(p, phase, splits, slot0, direct, early, st);
 }
 
 }  // namespace paged
