@@ -118,7 +118,15 @@ static int launch(Kernel kernel, const Attn& p, int phase, int splits, int two, 
       return launch_tc(p, a, st);
     }
   }
-  if (kernel == kRows) return launch_rows<T>(p, phase, splits, slot0, direct, early, st);
+  if (kernel == kRows) {
+    RowsArgs a = {};
+    a.phase = phase;
+    a.splits = splits;
+    a.slot0 = slot0;
+    a.direct = direct;
+    a.early = early;
+    return launch_rows<T>(p, a, st);
+  }
   return launch_simt<T>(p, phase, splits, slot0, direct, st);
 }
 
@@ -274,6 +282,11 @@ int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* o
   p.K = (int)kv->kv_heads;
   p.share = (int)(H / kv->kv_heads);
   p.D = (int)kv->head_dim;
+  p.by_page = gpt::paged::FastDiv(p.page);
+  p.by_K = gpt::paged::FastDiv(p.K);
+  p.by_share = gpt::paged::FastDiv(p.share);
+  p.by_rows = gpt::paged::FastDiv((int64_t)p.T * p.share);
+  p.by_per = gpt::paged::FastDiv(p.per);
   p.scale_log2 = scale * gpt::paged::kLog2e;
   const gpt::paged::Kernel best = dtype == GPT_BF16 && gpt::paged::tc_eligible(p)              ? gpt::paged::kTc
                                   : gpt::paged::rows_eligible(p, dtype == GPT_BF16 ? 2 : 4) ? gpt::paged::kRows

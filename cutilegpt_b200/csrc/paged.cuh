@@ -17,6 +17,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 // those of a group follow each other sequence by sequence.
 enum Phase { kPrefix = 0, kOwn = 1, kAll = 2 };
 
+// Division of 0 <= n < 2^31 by a number that the host knows: q = n m >> (31 + s) with s = ceil(log2 d),
+// m = ceil(2^(31 + s) / d) < 2^32; m d exceeds 2^(31 + s) by less than 2^s, too little to change q. A few
+// clocks, where a division by a variable is about a hundred, and a launch's first loads wait for several.
+struct FastDiv {
+  uint32_t d, m, s;
+  FastDiv() = default;
+  explicit FastDiv(int64_t div) : d((uint32_t)div), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ int div(int n) const { return (int)(((uint64_t)(uint32_t)n * m) >> (31 + s)); }
+  __device__ __forceinline__ int mod(int n) const { return n - div(n) * (int)d; }
+};
+
 struct Attn {
   const void* q;
   void* out;
@@ -36,12 +50,24 @@ struct Attn {
   int B, T, H, K, share;    // share = H / K
   int per;                  // sequences of a group (B without groups)
   int D;
+  FastDiv by_page, by_K, by_share, by_rows, by_per;   // by_rows: T * share, the rows of a sequence
   float scale_log2;
   // Partial results, slot by slot: acc [slot][row][D] (sum of 2^(s - m) v), ml [slot][row] (m, sum of
   // 2^(s - m)), row = (b * T + t) * H + h. Prefix parts are slots [0, n_pre), own parts n_pre ...
   float* acc;
   float2* ml;
   int n_pre, n_own;
+};
+
+// Row r of a phase's row space: sequence, token and head.
+struct Row {
+  int b, t, h;
+  __device__ __forceinline__ Row(const Attn& p, int b0, int kh, int r) {
+    const int i = p.by_rows.div(r), rr = r - i * (int)p.by_rows.d;
+    t = p.by_share.div(rr);
+    b = b0 + i;
+    h = kh * p.share + rr - t * p.share;
+  }
 };
 
 __device__ __forceinline__ int64_t row_id(const Attn& p, int b, int t, int h) {
@@ -78,7 +104,7 @@ struct Keys {
   int n_pre, n_own;
   __device__ Keys(const Attn& p, int phase, int seq_or_group) {
     const int b = phase == kPrefix ? seq_or_group * p.per : seq_or_group;
-    const int g = b / p.per;
+    const int g = phase == kPrefix ? seq_or_group : p.by_per.div(b);
     n_pre = phase == kOwn ? 0 : prefix_len(p, g);
     n_own = phase == kPrefix ? 0 : own_len(p, b);
     pre = p.ptable + (int64_t)g * p.ld_ptable;
@@ -89,8 +115,9 @@ struct Keys {
   __device__ int64_t offset(const Attn& p, int j, int kh) const {
     const bool own_part = j >= n_pre;
     const int i = own_part ? j - n_pre : j;
-    const int id = page_id((own_part ? own : pre)[i / p.page], p.n_pages);
-    return id < 0 ? -1 : id * p.page_stride + kh * p.head_stride + (int64_t)(i % p.page) * p.slot_stride;
+    const int at = p.by_page.div(i);
+    const int id = page_id((own_part ? own : pre)[at], p.n_pages);
+    return id < 0 ? -1 : id * p.page_stride + kh * p.head_stride + (int64_t)(i - at * p.page) * p.slot_stride;
   }
 };
 

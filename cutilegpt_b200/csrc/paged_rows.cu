@@ -142,6 +142,16 @@ __device__ __forceinline__ void join4(const Attn& p, int first, int n, int64_t r
     }
   }
 }
+__device__ __forceinline__ float4 peer_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 peer_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, float4 v) {
   if constexpr (sizeof(T) == 4)
@@ -150,34 +160,36 @@ __device__ __forceinline__ void store4(T* dst, float4 v) {
     *reinterpret_cast<uint2*>(dst) = make_uint2(tc::pack2_bf16(v.x, v.y), tc::pack2_bf16(v.z, v.w));
 }
 
+struct RowsArgs {
+  int phase, splits, slot0, direct, early;
+  int ctas_log2;            // CTAs of a cluster
+  FastDiv by_splits, by_blocks;
+};
+
 template <typename T, int DP, int W>
-__global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_kernel(const Attn p, int phase, int splits,
-                                                                                     int blocks, int slot0, int direct,
-                                                                                     int early) {
+__global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_kernel(const Attn p, const RowsArgs a) {
   using C = Rows<T, DP, W>;
   constexpr bool kWide = C::kWide;
   constexpr int KS = C::kKeys, kPer = 16 / (int)sizeof(T), kChunks = DP / kPer, kLoads = KS * kChunks / 32;
   constexpr int kTile = C::kTile, kRing = C::kRing;
   extern __shared__ __align__(128) uint8_t rows_smem_dyn[];
-  // With `early` the launch before is this call's prefix launch, whose every CTA has waited for all
+  // With early the launch before is this call's prefix launch, whose every CTA has waited for all
   // that came before it: what is read and written here is then safe, but for the prefix's partial results.
-  if (!early) pdl_wait();
+  if (!a.early) pdl_wait();
   pdl_trigger();
-  int item = blockIdx.x;
-  const int split = item % splits;
-  item /= splits;
-  const int block = item % blocks;
-  item /= blocks;
-  const int kh = item % p.K, who = item / p.K;
-  const int b0 = phase == kPrefix ? who * p.per : who;
-  const int rs = p.T * p.share;                       // rows of a sequence
-  const int rows = rs * (phase == kPrefix ? p.per : 1);
+  const int ctas = 1 << a.ctas_log2, rank = (int)blockIdx.x & (ctas - 1);
+  int item = (int)(blockIdx.x >> a.ctas_log2);
+  const int split_item = a.by_splits.div(item), split = item - split_item * a.splits;
+  const int block_item = a.by_blocks.div(split_item), block = split_item - block_item * (int)a.by_blocks.d;
+  const int who = p.by_K.div(block_item), kh = block_item - who * p.K;
+  const int b0 = a.phase == kPrefix ? who * p.per : who;
+  const int rows = (int)p.by_rows.d * (a.phase == kPrefix ? p.per : 1);
   const int r0 = block * kRowTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
-  const Keys keys(p, phase, who);
+  const Keys keys(p, a.phase, who);
   const int n = keys.n();
-  const int chunk = ((n + splits - 1) / splits + KS - 1) / KS * KS;
-  const int j0 = min(n, split * chunk);
+  const int chunk = ((a.by_splits.div(n + (a.splits << a.ctas_log2) - 1) >> a.ctas_log2) + KS - 1) / KS * KS;
+  const int j0 = min(n, (split * ctas + rank) * chunk);
   int j1 = min(n, j0 + chunk);
 
   // rows lane / 4 and lane / 4 + 8 of the tile
@@ -189,12 +201,12 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   for (int h = 0; h < 2; ++h) {
     const int r = r0 + lane / 4 + 8 * h;
     live[h] = r < rows;
-    const int b = b0 + (live[h] ? r / rs : 0), rr = live[h] ? r % rs : 0, t = rr / p.share;
-    const int last = keys.n_own - p.T + t;            // own key; below 0 the row is padding and sees nothing
-    seen[h] = !live[h] ? 0 : phase == kPrefix ? n : last < 0 ? 0 : keys.n_pre + last + 1;
+    const Row at(p, b0, kh, live[h] ? r : r0);
+    const int last = keys.n_own - p.T + at.t;         // own key; below 0 the row is padding and sees nothing
+    seen[h] = !live[h] ? 0 : a.phase == kPrefix ? n : last < 0 ? 0 : keys.n_pre + last + 1;
     most = max(most, seen[h]);
     if (live[h]) least = min(least, seen[h]);
-    src[h] = (const T*)p.q + b * p.q_b + (int64_t)(kh * p.share + rr % p.share) * p.q_h + t * p.q_t;
+    src[h] = (const T*)p.q + at.b * p.q_b + at.h * p.q_h + at.t * p.q_t;
   }
   j1 = min(j1, (int)__reduce_max_sync(0xffffffffu, (unsigned)most));
   least = min(j1, (int)__reduce_min_sync(0xffffffffu, (unsigned)least));
@@ -207,21 +219,21 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   const int steps = j1 > j0 + warp * KS ? (j1 - j0 - warp * KS + W * KS - 1) / (W * KS) : 0;
   // lane i holds the offsets of keys i, i + 32, ... of a step, -1 where there is none
   constexpr int kOffs = (KS + 31) / 32;
-  int64_t off[kOffs];
-  auto locate = [&](int s) {
+  int64_t off[kRing][kOffs];                       // the first steps' are looked up side by side
+  auto locate = [&](int s, int64_t (&to)[kOffs]) {
 #pragma unroll
     for (int i = 0; i < kOffs; ++i) {
       const int in = lane + 32 * i, j = j0 + (s * W + warp) * KS + in;
-      off[i] = in < KS && s < steps && j < j1 ? keys.offset(p, j, kh) : -1;
+      to[i] = in < KS && s < steps && j < j1 ? keys.offset(p, j, kh) : -1;
     }
   };
-  auto fetch = [&](int s) {
+  auto fetch = [&](int s, const int64_t (&from)[kOffs]) {
     const uint32_t dst = ring + (uint32_t)(s % kRing) * (2 * kTile);
     const int c = lane % kChunks;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int r = i * (32 / kChunks) + lane / kChunks;
-      const int64_t o = __shfl_sync(0xffffffffu, off[i * (32 / kChunks) / 32], r & 31);
+      const int64_t o = __shfl_sync(0xffffffffu, from[i * (32 / kChunks) / 32], r & 31);
       if (c * kPer < p.D) {
         const int64_t at = (o < 0 ? 0 : o) + c * kPer;
         cp_async16(dst + swz<T, DP>(r, c), (const T*)p.k + at, o >= 0);
@@ -230,11 +242,10 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     }
     cp_commit();
   };
-  for (int s = 0; s < kRing - 1; ++s) {
-    locate(s);
-    fetch(s);
-  }
-  locate(kRing - 1);
+#pragma unroll
+  for (int s = 0; s < kRing; ++s) locate(s, off[s]);
+#pragma unroll
+  for (int s = 0; s < kRing - 1; ++s) fetch(s, off[s]);
 
   // Q in the A fragments, with kQShared in shared memory as [step][lane]
   uint4* sq = reinterpret_cast<uint4*>(rows_smem_dyn);
@@ -253,13 +264,13 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
       if (C::kQShared && k % W != warp) continue;
-      uint32_t a[4];
+      uint32_t f[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = k * 16 + (i >> 1) * 8 + quad * 2;
-        a[i] = live[i & 1] && d < p.D ? *reinterpret_cast<const uint32_t*>(src[i & 1] + d) : 0u;
+        f[i] = live[i & 1] && d < p.D ? *reinterpret_cast<const uint32_t*>(src[i & 1] + d) : 0u;
       }
-      const uint4 x = make_uint4(a[0], a[1], a[2], a[3]);
+      const uint4 x = make_uint4(f[0], f[1], f[2], f[3]);
       if (C::kQShared)
         sq[k * 32 + lane] = x;
       else
@@ -267,9 +278,9 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     }
   }
   if (C::kQShared) __syncthreads();
-  auto q_frag = [&](int k, uint32_t (&a)[4]) {
+  auto q_frag = [&](int k, uint32_t (&f)[4]) {
     const uint4 x = C::kQShared ? sq[k * 32 + lane] : qf[C::kQShared ? 0 : k];
-    a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+    f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
   };
 
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[DP / 8][4];
@@ -280,8 +291,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   for (int s = 0; s < steps; ++s) {
     cp_wait<kRing - 2>();
     __syncwarp();
-    fetch(s + kRing - 1);      // into the slot of step s - 1, which every lane has left
-    locate(s + kRing);         // the table read is on its way while this step computes
+    fetch(s + kRing - 1, off[kRing - 1]);   // into the slot of step s - 1, which every lane has left
+    locate(s + kRing, off[kRing - 1]);      // the table read is on its way while this step computes
     const uint32_t sk = ring + (uint32_t)(s % kRing) * (2 * kTile), sv = sk + kTile;
     const int j = j0 + (s * W + warp) * KS;
     float sc[KS / 8][4];
@@ -309,14 +320,14 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     } else {
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k) {
-        uint32_t a[4];
-        q_frag(k, a);
+        uint32_t f[4];
+        q_frag(k, f);
 #pragma unroll
         for (int i = 0; i < KS / 16; ++i) {
           uint32_t kb[4];
           ldsm4(sk + swz<T, DP>(i * 16 + (lane >> 4) * 8 + (lane & 7), k * 2 + ((lane >> 3) & 1)), kb);
-          mma16816(sc[2 * i], a, kb[0], kb[1]);
-          mma16816(sc[2 * i + 1], a, kb[2], kb[3]);
+          mma16816(sc[2 * i], f, kb[0], kb[1]);
+          mma16816(sc[2 * i + 1], f, kb[2], kb[3]);
         }
       }
     }
@@ -338,18 +349,18 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * p.scale_log2;
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
-      float a[2];
+      float by[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float mn = fmaxf(m[h], mx[h]);
-        a[h] = mn == -INFINITY ? 1.f : exp2f(m[h] - mn);
+        by[h] = mn == -INFINITY ? 1.f : exp2f(m[h] - mn);
         m[h] = mn;
-        l[h] *= a[h];
+        l[h] *= by[h];
       }
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[i][k] *= a[k >> 1];
+        for (int k = 0; k < 4; ++k) o[i][k] *= by[k >> 1];
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) base[h] = m[h] == -INFINITY ? 0.f : m[h];   // a row without keys so far: every 2^(s - base) is 0
@@ -424,40 +435,59 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
         *reinterpret_cast<float2*>(dst + i * 8 + quad * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
     }
   }
-  __syncthreads();
-  if (early) pdl_wait();   // the prefix launch's partial results; its end, for whatever comes after this launch
+  if (ctas > 1)
+    tc::cluster_barrier();
+  else
+    __syncthreads();
+  if (a.early) pdl_wait();   // the prefix launch's partial results; its end, for whatever comes after this launch
+  const uint32_t my_o = (uint32_t)__cvta_generic_to_shared(sm_o), my_ml = (uint32_t)__cvta_generic_to_shared(sm_ml);
   const int n_live = min(kRowTile, rows - r0), quads = p.D / 4;
-  for (int i = threadIdx.x; i < n_live * quads; i += blockDim.x) {
+  for (int i = threadIdx.x + rank * blockDim.x; i < n_live * quads; i += blockDim.x * ctas) {
     const int rl = i / quads, d = i % quads * 4, r = r0 + rl;
     float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) top = fmaxf(top, sm_ml[w * kRowTile + rl].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < ctas; ++c) {   // in rank order: the same sums every time
+      const uint32_t o_at = tc::cluster_addr(my_o, (uint32_t)c) + (uint32_t)(rl * DP + d) * 4;
+      const uint32_t ml_at = tc::cluster_addr(my_ml, (uint32_t)c) + (uint32_t)rl * 8;
+      float2 ml[W];
+      float4 v[W];
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-      const float2 ml = sm_ml[w * kRowTile + rl];
-      const float c = ml.y == 0.f ? 0.f : exp2f(ml.x - top);
-      const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * kRowTile + rl) * DP + d);
-      sum = fmaf(ml.y, c, sum);
-      acc.x = fmaf(v.x, c, acc.x);
-      acc.y = fmaf(v.y, c, acc.y);
-      acc.z = fmaf(v.z, c, acc.z);
-      acc.w = fmaf(v.w, c, acc.w);
+      for (int w = 0; w < W; ++w) {
+        ml[w] = peer_f2(ml_at + w * kRowTile * 8);
+        v[w] = peer_f4(o_at + w * kRowTile * DP * 4);
+      }
+      float mx = top;
+#pragma unroll
+      for (int w = 0; w < W; ++w) mx = fmaxf(mx, ml[w].x);
+      const float by = sum == 0.f ? 0.f : exp2f(top - mx);
+      top = mx;
+      sum *= by;
+      acc.x *= by, acc.y *= by, acc.z *= by, acc.w *= by;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float f = ml[w].y == 0.f ? 0.f : exp2f(ml[w].x - mx);
+        sum = fmaf(ml[w].y, f, sum);
+        acc.x = fmaf(v[w].x, f, acc.x);
+        acc.y = fmaf(v[w].y, f, acc.y);
+        acc.z = fmaf(v[w].z, f, acc.z);
+        acc.w = fmaf(v[w].w, f, acc.w);
+      }
     }
-    const int b = b0 + r / rs, t = r % rs / p.share, h = kh * p.share + r % rs % p.share;
-    const int64_t row = row_id(p, b, t, h);
-    if (direct) {
-      const bool padding = keys.n_own - p.T + t < 0;
+    const Row at(p, b0, kh, r);
+    const int64_t row = row_id(p, at.b, at.t, at.h);
+    if (a.direct) {
+      const bool padding = keys.n_own - p.T + at.t < 0;
       if (!padding && p.n_pre > 0) join4(p, 0, p.n_pre, row, d, top, sum, acc);
       const float inv = padding ? 0.f : 1.f / sum;
-      store4((T*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d,
+      store4((T*)p.out + at.b * p.o_b + at.h * p.o_h + at.t * p.o_t + d,
              padding ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     } else {
-      const int64_t at = (int64_t)(slot0 + split) * p.B * p.T * p.H + row;
-      if (d == 0) p.ml[at] = make_float2(top, sum);
-      if (sum != 0.f) *reinterpret_cast<float4*>(p.acc + at * p.D + d) = acc;
+      const int64_t part = (int64_t)(a.slot0 + split) * p.B * p.T * p.H + row;
+      if (d == 0) p.ml[part] = make_float2(top, sum);
+      if (sum != 0.f) *reinterpret_cast<float4*>(p.acc + part * p.D + d) = acc;
     }
   }
+  if (ctas > 1) tc::cluster_barrier();   // the others have read this CTA's shared memory
 }
 
 // Whether the kernel serves the call: 16-byte rows of keys and values, pairs of q for bf16, quads of out.
@@ -474,7 +504,7 @@ static bool rows_eligible(const Attn& p, int size) {
 }
 
 template <typename T, int DP, int W>
-static int launch_rows_w(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+static int launch_rows_w(const Attn& p, RowsArgs a, cudaStream_t st) {
   using C = Rows<T, DP, W>;
   static bool done[64] = {false};
   static std::mutex mu;
@@ -488,29 +518,34 @@ static int launch_rows_w(const Attn& p, int phase, int splits, int slot0, int di
       done[dev] = true;
     }
   }
-  const int64_t rows = (int64_t)p.T * p.share * (phase == kPrefix ? p.per : 1);
+  const int64_t rows = (int64_t)p.T * p.share * (a.phase == kPrefix ? p.per : 1);
   const int64_t blocks = (rows + kRowTile - 1) / kRowTile;
-  const int64_t grid = blocks * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
+  const int64_t grid = (blocks * a.splits * p.K * (a.phase == kPrefix ? p.B / p.per : p.B)) << a.ctas_log2;
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
-  launch_pdl(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, phase, splits, (int)blocks,
-             slot0, direct, early);
+  a.by_splits = FastDiv(a.splits);
+  a.by_blocks = FastDiv(blocks);
+  if (a.ctas_log2 > 0)
+    launch_pdl_cluster(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, 1u << a.ctas_log2, p, a);
+  else
+    launch_pdl(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, a);
   return launch_status("paged_rows");
 }
 
 template <typename T, int DP>
-static int launch_rows_dp(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+static int launch_rows_dp(const Attn& p, RowsArgs a, cudaStream_t st) {
   static const char* e = getenv("ROWS_W");
-  return e && *e == '2' ? launch_rows_w<T, DP, 2>(p, phase, splits, slot0, direct, early, st)
-                        : launch_rows_w<T, DP, 4>(p, phase, splits, slot0, direct, early, st);
+  static const char* f = getenv("ROWS_S");
+  a.ctas_log2 = f ? atoi(f) : 0;
+  return e && *e == '2' ? launch_rows_w<T, DP, 2>(p, a, st) : launch_rows_w<T, DP, 4>(p, a, st);
 }
 
 template <typename T>
-static int launch_rows(const Attn& p, int phase, int splits, int slot0, int direct, int early, cudaStream_t st) {
+static int launch_rows(const Attn& p, const RowsArgs& a, cudaStream_t st) {
   if constexpr (sizeof(T) == 2)
-    if (p.D <= 16) return launch_rows_dp<T, 16>(p, phase, splits, slot0, direct, early, st);
-  if (p.D <= 32) return launch_rows_dp<T, 32>(p, phase, splits, slot0, direct, early, st);
-  if (p.D <= 64) return launch_rows_dp<T, 64>(p, phase, splits, slot0, direct, early, st);
-  return launch_rows_dp<T, 128>(p, phase, splits, slot0, direct, early, st);
+    if (p.D <= 16) return launch_rows_dp<T, 16>(p, a, st);
+  if (p.D <= 32) return launch_rows_dp<T, 32>(p, a, st);
+  if (p.D <= 64) return launch_rows_dp<T, 64>(p, a, st);
+  return launch_rows_dp<T, 128>(p, a, st);
 }
 
 }  // namespace paged

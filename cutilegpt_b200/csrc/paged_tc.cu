@@ -75,6 +75,7 @@ struct TcArgs {
   int phase, splits, blocks, slot0, direct, early, two;
   int tile;   // keys of a tile
   int box;    // keys of a TMA box
+  FastDiv by_splits, by_blocks, by_tile;
 };
 
 template <int D>
@@ -97,22 +98,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
 
   if (!a.early) pdl_wait();   // see paged_rows.cu
   pdl_trigger();
-  int item = blockIdx.x;
-  const int split = item % a.splits;
-  item /= a.splits;
-  const int block = item % a.blocks;
-  item /= a.blocks;
-  const int kh = item % p.K, who = item / p.K;
+  const int split_item = a.by_splits.div((int)blockIdx.x), split = (int)blockIdx.x - split_item * a.splits;
+  const int block_item = a.by_blocks.div(split_item), block = split_item - block_item * a.blocks;
+  const int who = p.by_K.div(block_item), kh = block_item - who * p.K;
   const int b0 = a.phase == kPrefix ? who * p.per : who;
-  const int rs = p.T * p.share;
-  const int rows = rs * (a.phase == kPrefix ? p.per : 1);
+  const int rows = (int)p.by_rows.d * (a.phase == kPrefix ? p.per : 1);
   const int r0 = block * (a.two ? 256 : 128);
   const Keys keys(p, a.phase, who);
   // own keys that the block's last row sees
   const int r_last = min(rows, r0 + (a.two ? 256 : 128)) - 1;
-  const int n_own = a.phase == kPrefix ? 0 : max(0, keys.n_own - p.T + r_last / p.share + 1);
-  const int nt_pre = (keys.n_pre + a.tile - 1) / a.tile, nt = nt_pre + (n_own + a.tile - 1) / a.tile;
-  const int per_split = (nt + a.splits - 1) / a.splits;
+  const int n_own = a.phase == kPrefix ? 0 : max(0, keys.n_own - p.T + p.by_share.div(r_last) + 1);
+  const int nt_pre = a.by_tile.div(keys.n_pre + a.tile - 1), nt = nt_pre + a.by_tile.div(n_own + a.tile - 1);
+  const int per_split = a.by_splits.div(nt + a.splits - 1);
   const int t0 = min(nt, split * per_split), n_tiles = min(nt, t0 + per_split) - t0;
   // pipelines with work, and the consumers of a ring slot
   const int pipes = n_tiles == 0 ? 0 : a.two ? (r0 + 128 < rows ? 2 : 1) : (n_tiles > 1 ? 2 : 1);
@@ -159,11 +156,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       const int t = t0 + i;
       const bool own = t >= nt_pre;
       const int at = (own ? t - nt_pre : t) * a.tile, valid = min(a.tile, (own ? n_own : keys.n_pre) - at);
-      boxes = (valid + a.box - 1) / a.box;
+      boxes = p.page <= 128 ? p.by_page.div(valid + a.box - 1) : 1;   // a box is a page, or 128 keys of one
       if (lane >= boxes) return -1;
-      const int pos = at + lane * a.box;
-      slot = pos % p.page;
-      const int id = page_id((own ? keys.own : keys.pre)[pos / p.page], p.n_pages);
+      const int pos = at + lane * a.box, page = p.by_page.div(pos);
+      slot = pos - page * p.page;
+      const int id = page_id((own ? keys.own : keys.pre)[page], p.n_pages);
       return id < 0 ? p.n_pages : id;   // past the pool: the map's fill value
     };
     int slot = 0, boxes = 0, id = n_tiles ? look(0, slot, boxes) : -1;
@@ -266,7 +263,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     uint64_t* pb = pipe_bars + 6 * pipe;
     const int r = r0 + (a.two ? pipe * 128 : 0) + rl;
     const bool live = r < rows;
-    const int b = b0 + (live ? r / rs : 0), rr = live ? r % rs : 0, t = rr / p.share, h = kh * p.share + rr % p.share;
+    const Row at_row(p, b0, kh, live ? r : r0);
+    const int b = at_row.b, t = at_row.t, h = at_row.h;
     // Q into its tile (with two == 0 by pipeline 0 for both)
     if (pipes > 0 && (pipe == 0 || a.two)) {
       uint8_t* dst = sQ + (a.two ? pipe : 0) * C::kTile + rl * 128;
@@ -512,6 +510,9 @@ static int launch_tc_d(const Attn& p, TcArgs a, cudaStream_t st) {
   const int64_t grid = blocks * a.splits * p.K * (a.phase == kPrefix ? p.B / p.per : p.B);
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
   a.blocks = (int)blocks;
+  a.by_splits = FastDiv(a.splits);
+  a.by_blocks = FastDiv(blocks);
+  a.by_tile = FastDiv(a.tile);
   launch_pdl(paged_tc_kernel<D>, dim3((unsigned)grid), dim3(kTcThreads), Tc<D>::kSmem, st, mk, mv, p, a);
   return launch_status("paged_tc");
 }
