@@ -251,30 +251,43 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   uint4* sq = reinterpret_cast<uint4*>(rows_smem_dyn);
   uint4 qf[C::kQShared ? 1 : C::kQSteps];
   if constexpr (kWide) {
-    for (int k = warp; k < DP / 8; k += W) {
-      // the contraction step's elements of this lane: 16 (k / 2) + 4 quad + 2 (k % 2) and the next one
-      const int d = 16 * (k / 2) + 4 * quad + 2 * (k % 2);
+    constexpr int kMine = (DP / 8 + W - 1) / W;      // contraction steps of this warp, all loads first
+    float x[kMine][4];
+#pragma unroll
+    for (int u = 0; u < kMine; ++u) {
+      // the step's elements of this lane: 16 (k / 2) + 4 quad + 2 (k % 2) and the next one
+      const int k = warp + u * W, d = 16 * (k / 2) + 4 * quad + 2 * (k % 2);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[u][i] = live[i & 1] && d + (i >> 1) < p.D ? src[i & 1][d + (i >> 1)] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < kMine; ++u) {
+      const int k = warp + u * W;
       uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) split_tf32(live[i & 1] && d + (i >> 1) < p.D ? src[i & 1][d + (i >> 1)] : 0.f, hi[i], lo[i]);
+      for (int i = 0; i < 4; ++i) split_tf32(x[u][i], hi[i], lo[i]);
       sq[2 * k * 32 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       sq[(2 * k + 1) * 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   } else {
-#pragma unroll
-    for (int k = 0; k < DP / 16; ++k) {
-      if (C::kQShared && k % W != warp) continue;
+    auto load = [&](int k) {
       uint32_t f[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int d = k * 16 + (i >> 1) * 8 + quad * 2;
         f[i] = live[i & 1] && d < p.D ? *reinterpret_cast<const uint32_t*>(src[i & 1] + d) : 0u;
       }
-      const uint4 x = make_uint4(f[0], f[1], f[2], f[3]);
-      if (C::kQShared)
-        sq[k * 32 + lane] = x;
-      else
-        qf[k] = x;
+      return make_uint4(f[0], f[1], f[2], f[3]);
+    };
+    if constexpr (C::kQShared) {
+      uint4 x[DP / 16 / W];
+#pragma unroll
+      for (int u = 0; u < DP / 16 / W; ++u) x[u] = load(warp + u * W);
+#pragma unroll
+      for (int u = 0; u < DP / 16 / W; ++u) sq[(warp + u * W) * 32 + lane] = x[u];
+    } else {
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) qf[k] = load(k);
     }
   }
   if (C::kQShared) __syncthreads();

@@ -269,9 +269,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     if (pipes > 0 && (pipe == 0 || a.two)) {
       uint8_t* dst = sQ + (a.two ? pipe : 0) * C::kTile + rl * 128;
       const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + b * p.q_b + (int64_t)h * p.q_h + t * p.q_t);
+      uint4 x[D / 8];   // all of the row's loads before the first store
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) x[c] = live ? src[c] : uint4{};
 #pragma unroll
       for (int c = 0; c < D / 8; ++c)
-        *reinterpret_cast<uint4*>(dst + (c / 8) * kPanel + (((c & 7) ^ (rl & 7)) << 4)) = live ? src[c] : uint4{};
+        *reinterpret_cast<uint4*>(dst + (c / 8) * kPanel + (((c & 7) ^ (rl & 7)) << 4)) = x[c];
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_addr(&pb[0]));
