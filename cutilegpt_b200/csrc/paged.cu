@@ -70,15 +70,14 @@ static void plan_launch(Kernel kernel, int64_t rows, int64_t items, int64_t keys
   const int64_t tiles128 = (rows + 127) / 128;
   *two = kernel == kTc && tiles128 > 1 && tiles128 != 3;
   if (kernel == kTc) {
-    // one CTA on an SM: no more than fit at once, at least two tiles for a pipeline
+    // one CTA on an SM: no more than fit at once, a tile at least for a pipeline
     items *= (rows + (*two ? 255 : 127)) / (*two ? 256 : 128);
-    const int64_t most = (keys + (*two ? 255 : 511)) / (*two ? 256 : 512), want = sms / (items > 0 ? items : 1);
+    const int64_t tile = *two ? 128 : 256, most = (keys + tile - 1) / tile, want = sms / (items > 0 ? items : 1);
     *splits = (int)(want < 1 ? 1 : want < most ? want : most < 1 ? 1 : most);
-    *slots = *two ? *splits : 2 * *splits;
   } else {
     *splits = shares(items * ((rows + 15) / 16), keys, sms, 2, 128);
-    *slots = *splits;
   }
+  *slots = *splits;
 }
 
 // The plan for the best kernel allowed.
@@ -95,8 +94,9 @@ static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, Kernel best)
   if (pl.shared) plan_launch(pl.pre, rows * per, groups * kv->kv_heads, pre_keys, sms, &pl.pre_splits, &pl.pre_two, &pl.n_pre);
   plan_launch(pl.own, rows, kv->batch * kv->kv_heads, own_keys + (pl.shared ? 0 : pre_keys), sms, &pl.own_splits, &pl.own_two,
               &pl.n_own);
-  // one share: the kernel joins the prefix's slots itself and writes out (the tcgen05 kernel: where there are none)
-  if (pl.n_own == 1 && (pl.own != kTc || pl.n_pre == 0)) pl.n_own = 0;
+  // one share: the kernel joins the prefix's slots itself and writes out (the tcgen05 kernel: where there are none;
+  // the few-row kernel: as many as it has room for)
+  if (pl.n_own == 1 && (pl.own == kTc ? pl.n_pre == 0 : pl.own == kRows ? pl.n_pre <= kMaxSlots : true)) pl.n_own = 0;
   const int64_t parts = (int64_t)(pl.n_pre + pl.n_own) * kv->batch * T * H;
   pl.acc_floats = (parts * kv->head_dim + 3) / 4 * 4;
   pl.bytes = (pl.acc_floats + 2 * parts) * (int64_t)sizeof(float);
@@ -125,6 +125,14 @@ static int launch(Kernel kernel, const Attn& p, int phase, int splits, int two, 
     a.slot0 = slot0;
     a.direct = direct;
     a.early = early;
+    // Two warps a CTA where four would not fit at once and a share's keys are few: a CTA's start and end then
+    // weigh more than its steps, and smaller CTAs overlap more of them (B200, 768 and 1600 CTAs of up to 256
+    // keys, D = 64: 14 and 37 us, with four warps 21 and 42; 536 CTAs of up to 1024 keys, D = 128: 69, with four 56).
+    const int64_t rows = (int64_t)p.T * p.share * (phase == kPrefix ? p.per : 1);
+    const int64_t ctas = (rows + 15) / 16 * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
+    const int64_t share_keys = ((int64_t)(phase == kOwn ? 0 : p.pcap) + (phase == kPrefix ? 0 : p.cap)) / splits;
+    const int fit = (sizeof(T) == 4 ? 8 : p.D > 64 ? 12 : 16) / 4;
+    a.two_warps = ctas > (int64_t)fit * device_sm_count() && share_keys <= 512;
     return launch_rows<T>(p, a, st);
   }
   return launch_simt<T>(p, phase, splits, slot0, direct, st);

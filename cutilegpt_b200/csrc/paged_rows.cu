@@ -23,6 +23,7 @@ namespace gpt {
 namespace paged {
 
 constexpr int kRowTile = 16;
+constexpr int kMaxSlots = 32;    // prefix slots that the kernel joins itself
 
 template <typename T, int DP, int W>   // DP: head size padded to a power of two
 struct Rows {
@@ -36,7 +37,7 @@ struct Rows {
   static constexpr int kQSteps = kWide ? DP / 4 : DP / 16;     // uint4 of a lane
   static constexpr int kQ = kQShared ? kQSteps * 512 : 0;
   static constexpr int kRings = W * kRing * 2 * kTile;
-  static constexpr int kMerge = W * kRowTile * (DP + 2) * 4;
+  static constexpr int kMerge = W * kRowTile * (DP + 2) * 4 + kRowTile * kMaxSlots * 8;
   static constexpr int kSmem = (kRings > kMerge ? kRings : kMerge) + kQ;
 };
 
@@ -109,49 +110,6 @@ __device__ __forceinline__ void mma_split(float (&c)[4], const uint32_t (&ah)[4]
   mma1688(c, ah, h0, h1);
 }
 
-// One row's four columns joined with the partial slots first .. first + n - 1, eight at a time.
-__device__ __forceinline__ void join4(const Attn& p, int first, int n, int64_t row, int d, float& m, float& l, float4& acc) {
-  const int64_t rows = (int64_t)p.B * p.T * p.H;
-  for (int s0 = 0; s0 < n; s0 += 8) {
-    float2 o[8];
-    float4 v[8];
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const int64_t at = (int64_t)(first + min(s0 + s, n - 1)) * rows + row;
-      o[s] = __ldcg(p.ml + at);
-      v[s] = __ldcg(reinterpret_cast<const float4*>(p.acc + at * p.D + d));
-      if (s0 + s >= n) o[s].y = 0.f;
-    }
-    float top = l == 0.f ? -INFINITY : m;
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-      if (o[s].y != 0.f) top = fmaxf(top, o[s].x);
-    const float a = l == 0.f ? 0.f : exp2f(m - top);
-    m = top;
-    l *= a;
-    acc.x *= a, acc.y *= a, acc.z *= a, acc.w *= a;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      if (o[s].y == 0.f) continue;   // no keys: its accumulator was not written
-      const float w = exp2f(o[s].x - top);
-      l = fmaf(o[s].y, w, l);
-      acc.x = fmaf(v[s].x, w, acc.x);
-      acc.y = fmaf(v[s].y, w, acc.y);
-      acc.z = fmaf(v[s].z, w, acc.z);
-      acc.w = fmaf(v[s].w, w, acc.w);
-    }
-  }
-}
-__device__ __forceinline__ float4 peer_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 peer_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
-}
 template <typename T>
 __device__ __forceinline__ void store4(T* dst, float4 v) {
   if constexpr (sizeof(T) == 4)
@@ -162,7 +120,7 @@ __device__ __forceinline__ void store4(T* dst, float4 v) {
 
 struct RowsArgs {
   int phase, splits, slot0, direct, early;
-  int ctas_log2;            // CTAs of a cluster
+  int two_warps;            // CTAs of two warps, not four
   FastDiv by_splits, by_blocks;
 };
 
@@ -177,9 +135,7 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   // that came before it: what is read and written here is then safe, but for the prefix's partial results.
   if (!a.early) pdl_wait();
   pdl_trigger();
-  const int ctas = 1 << a.ctas_log2, rank = (int)blockIdx.x & (ctas - 1);
-  int item = (int)(blockIdx.x >> a.ctas_log2);
-  const int split_item = a.by_splits.div(item), split = item - split_item * a.splits;
+  const int split_item = a.by_splits.div((int)blockIdx.x), split = (int)blockIdx.x - split_item * a.splits;
   const int block_item = a.by_blocks.div(split_item), block = split_item - block_item * (int)a.by_blocks.d;
   const int who = p.by_K.div(block_item), kh = block_item - who * p.K;
   const int b0 = a.phase == kPrefix ? who * p.per : who;
@@ -188,8 +144,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
   const Keys keys(p, a.phase, who);
   const int n = keys.n();
-  const int chunk = ((a.by_splits.div(n + (a.splits << a.ctas_log2) - 1) >> a.ctas_log2) + KS - 1) / KS * KS;
-  const int j0 = min(n, (split * ctas + rank) * chunk);
+  const int chunk = (a.by_splits.div(n + a.splits - 1) + KS - 1) / KS * KS;
+  const int j0 = min(n, split * chunk);
   int j1 = min(n, j0 + chunk);
 
   // rows lane / 4 and lane / 4 + 8 of the tile
@@ -430,6 +386,7 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   __syncthreads();
   float* sm_o = reinterpret_cast<float*>(rows_smem_dyn + C::kQ);         // [warp][16][DP]
   float2* sm_ml = reinterpret_cast<float2*>(sm_o + W * kRowTile * DP);   // [warp][16]
+  float2* sm_w = sm_ml + W * kRowTile;                                   // [16][kMaxSlots]
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = lane / 4 + 8 * h;
@@ -448,59 +405,67 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
         *reinterpret_cast<float2*>(dst + i * 8 + quad * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
     }
   }
-  if (ctas > 1)
-    tc::cluster_barrier();
-  else
-    __syncthreads();
+  __syncthreads();
   if (a.early) pdl_wait();   // the prefix launch's partial results; its end, for whatever comes after this launch
-  const uint32_t my_o = (uint32_t)__cvta_generic_to_shared(sm_o), my_ml = (uint32_t)__cvta_generic_to_shared(sm_ml);
-  const int n_live = min(kRowTile, rows - r0), quads = p.D / 4;
-  for (int i = threadIdx.x + rank * blockDim.x; i < n_live * quads; i += blockDim.x * ctas) {
-    const int rl = i / quads, d = i % quads * 4, r = r0 + rl;
-    float top = -INFINITY, sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = 0; c < ctas; ++c) {   // in rank order: the same sums every time
-      const uint32_t o_at = tc::cluster_addr(my_o, (uint32_t)c) + (uint32_t)(rl * DP + d) * 4;
-      const uint32_t ml_at = tc::cluster_addr(my_ml, (uint32_t)c) + (uint32_t)rl * 8;
-      float2 ml[W];
-      float4 v[W];
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        ml[w] = peer_f2(ml_at + w * kRowTile * 8);
-        v[w] = peer_f4(o_at + w * kRowTile * DP * 4);
-      }
-      float mx = top;
-#pragma unroll
-      for (int w = 0; w < W; ++w) mx = fmaxf(mx, ml[w].x);
-      const float by = sum == 0.f ? 0.f : exp2f(top - mx);
-      top = mx;
-      sum *= by;
-      acc.x *= by, acc.y *= by, acc.z *= by, acc.w *= by;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float f = ml[w].y == 0.f ? 0.f : exp2f(ml[w].x - mx);
-        sum = fmaf(ml[w].y, f, sum);
-        acc.x = fmaf(v[w].x, f, acc.x);
-        acc.y = fmaf(v[w].y, f, acc.y);
-        acc.z = fmaf(v[w].z, f, acc.z);
-        acc.w = fmaf(v[w].w, f, acc.w);
-      }
-    }
-    const Row at(p, b0, kh, r);
+  // A row's parts: the prefix's slots and the CTA's warps, in that order. Everything that comes from global
+  // memory is asked for at once: the slots' (m, l) of all rows, by all threads, and the first slots'
+  // columns of the thread's first item.
+  const int n_live = min(kRowTile, rows - r0), quads = p.D / 4, n_pre = a.direct ? p.n_pre : 0;
+  const int64_t all_rows = (int64_t)p.B * p.T * p.H;
+  for (int i = threadIdx.x; i < n_live * n_pre; i += W * 32) {
+    const int rl = i / n_pre, s = i - rl * n_pre;
+    const Row at(p, b0, kh, r0 + rl);
+    sm_w[rl * kMaxSlots + s] = __ldcg(p.ml + s * all_rows + row_id(p, at.b, at.t, at.h));
+  }
+  bool first = true;
+#pragma unroll 1
+  for (int i = threadIdx.x; first || i < n_live * quads; i += W * 32) {
+    const bool mine = i < n_live * quads;            // the first round is everyone's, for its barrier
+    const int rl = mine ? i / quads : 0, d = mine ? (i - rl * quads) * 4 : 0;
+    const Row at(p, b0, kh, r0 + rl);
     const int64_t row = row_id(p, at.b, at.t, at.h);
+    const float* part = p.acc + row * p.D + d;
+    float4 v[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (mine && s < n_pre) v[s] = __ldcg(reinterpret_cast<const float4*>(part + s * all_rows * p.D));
+    if (first) __syncthreads();
+    first = false;
+    if (!mine) break;
+    const float2* slots = sm_w + rl * kMaxSlots;
+    float top = -INFINITY, sum = 0.f;
+    for (int s = 0; s < n_pre; ++s) top = slots[s].y != 0.f ? fmaxf(top, slots[s].x) : top;
+#pragma unroll
+    for (int u = 0; u < W; ++u) top = fmaxf(top, sm_ml[u * kRowTile + rl].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float2 ml, float4 x) {            // a part without keys has l = 0 and anything in x
+      const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - top);
+      if (w != 0.f) {
+        sum = fmaf(ml.y, w, sum);
+        acc.x = fmaf(x.x, w, acc.x);
+        acc.y = fmaf(x.y, w, acc.y);
+        acc.z = fmaf(x.z, w, acc.z);
+        acc.w = fmaf(x.w, w, acc.w);
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s < n_pre) add(slots[s], v[s]);
+#pragma unroll 4
+    for (int s = 8; s < n_pre; ++s) add(slots[s], __ldcg(reinterpret_cast<const float4*>(part + s * all_rows * p.D)));
+#pragma unroll
+    for (int u = 0; u < W; ++u)
+      add(sm_ml[u * kRowTile + rl], *reinterpret_cast<const float4*>(sm_o + (u * kRowTile + rl) * DP + d));
     if (a.direct) {
-      const bool padding = keys.n_own - p.T + at.t < 0;
-      if (!padding && p.n_pre > 0) join4(p, 0, p.n_pre, row, d, top, sum, acc);
-      const float inv = padding ? 0.f : 1.f / sum;
+      const float inv = sum == 0.f || keys.n_own - p.T + at.t < 0 ? 0.f : 1.f / sum;   // 0: padding
       store4((T*)p.out + at.b * p.o_b + at.h * p.o_h + at.t * p.o_t + d,
-             padding ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+             inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     } else {
-      const int64_t part = (int64_t)(a.slot0 + split) * p.B * p.T * p.H + row;
-      if (d == 0) p.ml[part] = make_float2(top, sum);
-      if (sum != 0.f) *reinterpret_cast<float4*>(p.acc + part * p.D + d) = acc;
+      const int64_t to = (int64_t)(a.slot0 + split) * all_rows + row;
+      if (d == 0) p.ml[to] = make_float2(top, sum);
+      *reinterpret_cast<float4*>(p.acc + to * p.D + d) = acc;
     }
   }
-  if (ctas > 1) tc::cluster_barrier();   // the others have read this CTA's shared memory
 }
 
 // Whether the kernel serves the call: 16-byte rows of keys and values, pairs of q for bf16, quads of out.
@@ -533,23 +498,17 @@ static int launch_rows_w(const Attn& p, RowsArgs a, cudaStream_t st) {
   }
   const int64_t rows = (int64_t)p.T * p.share * (a.phase == kPrefix ? p.per : 1);
   const int64_t blocks = (rows + kRowTile - 1) / kRowTile;
-  const int64_t grid = (blocks * a.splits * p.K * (a.phase == kPrefix ? p.B / p.per : p.B)) << a.ctas_log2;
+  const int64_t grid = blocks * a.splits * p.K * (a.phase == kPrefix ? p.B / p.per : p.B);
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
   a.by_splits = FastDiv(a.splits);
   a.by_blocks = FastDiv(blocks);
-  if (a.ctas_log2 > 0)
-    launch_pdl_cluster(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, 1u << a.ctas_log2, p, a);
-  else
-    launch_pdl(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, a);
+  launch_pdl(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, a);
   return launch_status("paged_rows");
 }
 
 template <typename T, int DP>
 static int launch_rows_dp(const Attn& p, RowsArgs a, cudaStream_t st) {
-  static const char* e = getenv("ROWS_W");
-  static const char* f = getenv("ROWS_S");
-  a.ctas_log2 = f ? atoi(f) : 0;
-  return e && *e == '2' ? launch_rows_w<T, DP, 2>(p, a, st) : launch_rows_w<T, DP, 4>(p, a, st);
+  return a.two_warps ? launch_rows_w<T, DP, 2>(p, a, st) : launch_rows_w<T, DP, 4>(p, a, st);
 }
 
 template <typename T>

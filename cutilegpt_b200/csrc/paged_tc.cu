@@ -9,8 +9,7 @@
 // warpgroup (one thread per row = TMEM lane) and one MMA-issuing lane work on
 //   two != 0: the same tiles, pipeline s on rows 128 s .. of the block, so that 256
 //             rows share one reading of the keys,
-//   two == 0: the same 128 rows, pipeline s on tiles s, s + 2, ... of the share, each with a
-//             partial result of its own,
+//   two == 0: the same 128 rows, pipeline s on tiles s, s + 2, ... of the share; the results are joined at the end,
 // so that one's products run while the other's softmax does. Per tile:
 //   S = Q Kᵀ      tcgen05.mma M=128 N=128 K=D -> TMEM
 //   softmax       the row's 128 scores are read into registers, masked (the row's keys end inside a
@@ -66,7 +65,7 @@ struct Tc {
   static constexpr int kPanels = D / 64;
   static constexpr int kTile = kPanels * kPanel;         // a Q, K or V tile
   static constexpr int kStages = D == 64 ? 5 : 2;        // of each ring: 160 or 128 KB in flight
-  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kStages * kTile + 512;
+  static constexpr int kSmem = 1024 + 2 * kTile + 2 * kStages * kTile + 512 + 256 * (int)sizeof(float2);
   static constexpr bool kAlias = D == 128;               // P in the columns of S
   static constexpr uint32_t kP = kAlias ? 0 : 128, kO = kAlias ? 128 : 192;
 };
@@ -94,6 +93,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
   uint64_t* pipe_bars = bars + 4 * ST;      // per pipeline: q_full, s_full, s_free, p_full (two halves), o_full
   uint64_t* turns = pipe_bars + 12;         // [pipeline][warp of the warpgroup]: its exponentials may begin
   uint32_t* tmem_slot = (uint32_t*)(turns + 8);
+  float2* ml_smem = (float2*)((uint8_t*)bars + 512);   // [pipeline][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (!a.early) pdl_wait();   // see paged_rows.cu
@@ -263,25 +263,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     uint64_t* pb = pipe_bars + 6 * pipe;
     const int r = r0 + (a.two ? pipe * 128 : 0) + rl;
     const bool live = r < rows;
-    const Row at_row(p, b0, kh, live ? r : r0);
-    const int b = at_row.b, t = at_row.t, h = at_row.h;
-    // Q into its tile (with two == 0 by pipeline 0 for both)
-    if (pipes > 0 && (pipe == 0 || a.two)) {
-      uint8_t* dst = sQ + (a.two ? pipe : 0) * C::kTile + rl * 128;
-      const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + b * p.q_b + (int64_t)h * p.q_h + t * p.q_t);
-      uint4 x[D / 8];   // all of the row's loads before the first store
+    int last;   // last own key of the row; below 0: padding
+    {
+      const Row at(p, b0, kh, live ? r : r0);
+      last = a.phase == kPrefix ? 0 : keys.n_own - p.T + at.t;
+      // Q into its tile (with two == 0 by pipeline 0 for both)
+      if (pipes > 0 && (pipe == 0 || a.two)) {
+        uint8_t* dst = sQ + (a.two ? pipe : 0) * C::kTile + rl * 128;
+        const uint4* src = reinterpret_cast<const uint4*>((const __nv_bfloat16*)p.q + at.b * p.q_b + at.h * p.q_h + at.t * p.q_t);
+        uint4 x[D / 8];   // all of the row's loads before the first store
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) x[c] = live ? src[c] : uint4{};
+        for (int c = 0; c < D / 8; ++c) x[c] = live ? src[c] : uint4{};
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c)
-        *reinterpret_cast<uint4*>(dst + (c / 8) * kPanel + (((c & 7) ^ (rl & 7)) << 4)) = x[c];
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&pb[0]));
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<uint4*>(dst + (c / 8) * kPanel + (((c & 7) ^ (rl & 7)) << 4)) = x[c];
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&pb[0]));
+      }
     }
     const uint32_t tm = *tmem_slot + (uint32_t)(pipe * 256) + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t tS = tm, tP = tm + C::kP, tO = tm + C::kO;
-    const int last = a.phase == kPrefix ? 0 : keys.n_own - p.T + t;   // last own key of the row; below 0: padding
     const int seen_own = live ? max(0, last + 1) : 0;
     const int seen_pre = live && (a.phase == kPrefix || last >= 0) ? keys.n_pre : 0;
     float m = -INFINITY, l = 0.f, top = -INFINITY;   // top: the largest scaled score so far
@@ -416,41 +418,72 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       if (ok && !mbar_wait(smem_addr(&pb[5]), C::kAlias ? 0u : (uint32_t)((g - 1) & 1))) ok = false;
       tc_fence_after();
     }
-    // the row's result: out, or its slot of partial results
+    // The row's result: out, or its slot of partial results. Two pipelines on the same rows see each
+    // other's (m, l) through shared memory and O in TMEM (same lanes), and write half the columns each.
+    float scale0 = 1.f, scale1 = 0.f;   // of this pipeline's O, of the other's
+    const bool shared_rows = !a.two && pipes == 2;
+    if (shared_rows) {
+      tc_fence_before();
+      ml_smem[pipe * 128 + rl] = make_float2(m, l);
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      tc_fence_after();
+      const float2 o = ml_smem[(1 - pipe) * 128 + rl];
+      const float to = fmaxf(m, o.x);
+      scale0 = l == 0.f ? 0.f : ex2(m - to);
+      scale1 = o.y == 0.f ? 0.f : ex2(o.x - to);
+      l = l * scale0 + o.y * scale1;
+      m = to;
+    }
     if (a.early) pdl_wait();
-    const int64_t row = row_id(p, b, t, h);
-    const int64_t slot = (int64_t)a.slot0 + (a.two ? split : 2 * split + pipe);
-    const int64_t at = slot * p.B * p.T * p.H + row;
-    const bool mine = live && (a.direct ? a.two != 0 || pipe == 0 : true);
-    const bool none = l == 0.f;
-    if (mine && !a.direct) p.ml[at] = make_float2(m, l);
-    const float inv = none ? 0.f : 1.f / l;
-    if (pipe < pipes) {
+    const Row to_row(p, b0, kh, live ? r : r0);
+    const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to_row.b, to_row.t, to_row.h);
+    const bool mine = live && (a.two || shared_rows || pipe == 0), none = l == 0.f;
+    if (mine && !a.direct && (a.two || pipe == 0)) p.ml[at] = make_float2(m, l);
+    if (a.direct) {
+      const float inv = none ? 0.f : 1.f / l;
+      scale0 *= inv;
+      scale1 *= inv;
+    }
+    auto put = [&](int c, const uint32_t (&o)[32]) {   // columns c .. c + 31 of the row
+      if (!mine) return;
+      if (a.direct) {
+        uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)p.out + to_row.b * p.o_b + to_row.h * p.o_h + to_row.t * p.o_t + c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t w[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            w[u] = none ? 0u : tc::pack2_bf16(__uint_as_float(o[8 * k + 2 * u]), __uint_as_float(o[8 * k + 2 * u + 1]));
+          dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else if (!none) {
+        uint4* dst = reinterpret_cast<uint4*>(p.acc + at * D + c);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+      }
+    };
+    if (shared_rows) {
+#pragma unroll 1
+      for (int c = pipe * (D / 2); c < (pipe + 1) * (D / 2); c += 32) {
+        uint32_t o[32], x[32];
+        tmem_ld32(tO + (uint32_t)c, o);
+        tmem_ld32((pipe == 0 ? tO + 256 : tO - 256) + (uint32_t)c, x);
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          o[k] = __float_as_uint(__uint_as_float(o[k]) * scale0 + __uint_as_float(x[k]) * scale1);
+        put(c, o);
+      }
+    } else {
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(tO + (uint32_t)c, o);
-        if (!mine) continue;
+        uint32_t o[32] = {};
+        if (pipe < pipes) tmem_ld32(tO + (uint32_t)c, o);
         if (a.direct) {
-          uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + c);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t w[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              w[u] = none ? 0u : tc::pack2_bf16(__uint_as_float(o[8 * k + 2 * u]) * inv, __uint_as_float(o[8 * k + 2 * u + 1]) * inv);
-            dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
-          }
-        } else if (!none) {
-          uint4* dst = reinterpret_cast<uint4*>(p.acc + at * D + c);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) dst[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * scale0);
         }
+        put(c, o);
       }
-    } else if (mine && a.direct) {   // no keys at all: rows of padding
-      uint4* dst = reinterpret_cast<uint4*>((__nv_bfloat16*)p.out + b * p.o_b + h * p.o_h + t * p.o_t);
-#pragma unroll
-      for (int k = 0; k < D / 8; ++k) dst[k] = uint4{};
     }
   }
   tc_fence_before();
