@@ -218,13 +218,13 @@ int gpt_paged_kv_append(const void* q, const int64_t* q_strides, const void* k, 
   p.T = (int)T;
   p.K = (int)kv->kv_heads;
   p.D = (int)kv->head_dim;
-  p.heads = (int)(2 * kv->kv_heads + (rot ? H : 0));
-  const int64_t tokens = kv->batch * T;
+  p.B = (int)kv->batch;
+  const int64_t heads = 2 * kv->kv_heads + (rot ? H : 0);
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == GPT_BF16)
-    return wide ? gpt::paged::launch_append<__nv_bfloat16, 8>(p, tokens, st)
-                : gpt::paged::launch_append<__nv_bfloat16, 1>(p, tokens, st);
-  return wide ? gpt::paged::launch_append<float, 4>(p, tokens, st) : gpt::paged::launch_append<float, 1>(p, tokens, st);
+    return wide ? gpt::paged::launch_append<__nv_bfloat16, 8>(p, heads, st)
+                : gpt::paged::launch_append<__nv_bfloat16, 1>(p, heads, st);
+  return wide ? gpt::paged::launch_append<float, 4>(p, heads, st) : gpt::paged::launch_append<float, 1>(p, heads, st);
 }
 
 int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H, const gpt_paged_kv* kv, int dtype) {

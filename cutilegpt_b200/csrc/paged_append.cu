@@ -35,43 +35,23 @@ struct Append {
   int64_t n_pos;
   int rot, interleaved;
   int T, K, D;
-  int heads;     // 2 K, or 2 K + H with rotation
-  int units;     // pairs of vectors of a head
-  int64_t total; // threads with work
+  int B;
+  int total;     // threads with work for a sequence: tokens x heads x pairs of vectors of a head
+  FastDiv by_heads, by_units, by_page;   // heads: 2 K, or 2 K + H with rotation
 };
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Vec {
   T e[V];
 };
 
+// One thread's share of sequence b.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) paged_append_kernel(const Append p) {
-  pdl_wait();
-  pdl_trigger();
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (id >= p.total) return;
-  const int64_t token_head = id / p.units;
-  const int u = (int)(id - token_head * p.units);
-  const int64_t token = token_head / p.heads;
-  int h = (int)(token_head - token * p.heads);
-  const int b = (int)(token / p.T), t = (int)(token - (int64_t)b * p.T);
+__device__ __forceinline__ void append_one(const Append& p, int b, int id) {
+  const int token_head = p.by_units.div(id), u = id - token_head * (int)p.by_units.d;
+  const int t = p.by_heads.div(token_head);
+  int h = token_head - t * (int)p.by_heads.d;
   const int kind = h < p.K ? 0 : h < 2 * p.K ? 1 : 2;   // key, value, query
-  if (kind) h -= kind * p.K;
-
-  const int pre = p.plens ? clamped_len(p.plens, b / p.per, p.pcap) : 0;
-  const int i = clamped_len(p.seq_lens, b, p.cap) - p.T + t;
-  const int64_t* s = kind == 0 ? p.k_s : kind == 1 ? p.v_s : p.q_s;
-  const T* src = (const T*)(kind == 0 ? p.k : kind == 1 ? p.v : p.q) + b * s[0] + h * s[1] + t * s[2];
-  T* dst;
-  if (kind == 2) {
-    dst = (T*)p.q_out + b * p.o_s[0] + h * p.o_s[1] + t * p.o_s[2];
-  } else {
-    if (i < 0) return;   // padding
-    const int pid = page_id(p.table[b * p.ld_table + i / p.page], p.n_pages);
-    if (pid < 0) return;
-    dst = (T*)(kind == 0 ? p.k_pages : p.v_pages) + pid * p.page_stride + h * p.head_stride +
-          (int64_t)(i % p.page) * p.slot_stride;
-  }
+  h -= kind * p.K;
 
   const int rot = kind == 1 ? 0 : p.rot, half = rot / 2;
   const bool halves = rot > 0 && !p.interleaved && u * V < half;
@@ -80,19 +60,35 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const Append p) {
   const int d1 = halves ? half + u * V : d0 + V;
   const bool second = d1 < p.D;
   using W = Vec<T, V>;
+  // the values are on their way while the length and the page are looked up
+  const int64_t* s = kind == 0 ? p.k_s : kind == 1 ? p.v_s : p.q_s;
+  const T* src = (const T*)(kind == 0 ? p.k : kind == 1 ? p.v : p.q) + b * s[0] + h * s[1] + t * s[2];
   W a = *reinterpret_cast<const W*>(src + d0), c = {};
   if (second) c = *reinterpret_cast<const W*>(src + d1);
+
+  const int pre = p.plens ? clamped_len(p.plens, b / p.per, p.pcap) : 0;
+  const int i = clamped_len(p.seq_lens, b, p.cap) - p.T + t;
+  T* dst;
+  if (kind == 2) {
+    dst = (T*)p.q_out + b * p.o_s[0] + h * p.o_s[1] + t * p.o_s[2];
+  } else {
+    if (i < 0) return;   // padding
+    const int page = p.by_page.div(i), pid = page_id(p.table[b * p.ld_table + page], p.n_pages);
+    if (pid < 0) return;
+    dst = (T*)(kind == 0 ? p.k_pages : p.v_pages) + pid * p.page_stride + h * p.head_stride +
+          (int64_t)(i - page * p.page) * p.slot_stride;
+  }
   if (d0 < rot) {
     const int64_t n = (int64_t)pre + i;
     const bool known = i >= 0 && n >= 0 && n < p.n_pos;
     if (i >= 0 && !known) record_device_error(GPT_DEVERR_INDEX);
     const float* cs = p.cos_sin + n * rot;
+    using F = Vec<float, V % 4 == 0 ? 4 : 1>;
+    constexpr int FV = sizeof(F) / sizeof(float);
     if (!known) {
       a = {};
       c = {};
     } else if (halves) {
-      using F = Vec<float, V % 4 == 0 ? 4 : 1>;
-      constexpr int FV = sizeof(F) / sizeof(float);
 #pragma unroll
       for (int j0 = 0; j0 < V; j0 += FV) {
         const F co = *reinterpret_cast<const F*>(cs + d0 + j0), si = *reinterpret_cast<const F*>(cs + half + d0 + j0);
@@ -106,14 +102,18 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const Append p) {
     } else {
       // 2 V neighbouring elements, V pairs; the pairs at and past rot stay
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (d0 + 2 * j >= rot) break;
-        T& e0 = 2 * j < V ? a.e[2 * j % V] : c.e[2 * j % V];
-        T& e1 = 2 * j + 1 < V ? a.e[(2 * j + 1) % V] : c.e[(2 * j + 1) % V];
-        const float x0 = Tr<T>::to_f(e0), x1 = Tr<T>::to_f(e1);
-        const float co = cs[d0 / 2 + j], si = cs[half + d0 / 2 + j];
-        e0 = Tr<T>::from_f(x0 * co - x1 * si);
-        e1 = Tr<T>::from_f(x0 * si + x1 * co);
+      for (int j0 = 0; j0 < V; j0 += FV) {
+        if (d0 + 2 * j0 >= rot) break;   // rot is a multiple of 2 FV where FV > 1
+        const F co = *reinterpret_cast<const F*>(cs + d0 / 2 + j0), si = *reinterpret_cast<const F*>(cs + half + d0 / 2 + j0);
+#pragma unroll
+        for (int j = 0; j < FV; ++j) {
+          const int e = 2 * (j0 + j);
+          T& e0 = e < V ? a.e[e % V] : c.e[e % V];
+          T& e1 = e + 1 < V ? a.e[(e + 1) % V] : c.e[(e + 1) % V];
+          const float x0 = Tr<T>::to_f(e0), x1 = Tr<T>::to_f(e1);
+          e0 = Tr<T>::from_f(x0 * co.e[j] - x1 * si.e[j]);
+          e1 = Tr<T>::from_f(x0 * si.e[j] + x1 * co.e[j]);
+        }
       }
     }
   } else if (kind == 2 && i < 0) {
@@ -128,13 +128,27 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const Append p) {
   if (second) *reinterpret_cast<W*>(dst + d1) = c;
 }
 
+constexpr int kAppendThreads = 128;
+
 template <typename T, int V>
-static int launch_append(Append p, int64_t tokens, cudaStream_t st) {
-  p.units = (p.D + 2 * V - 1) / (2 * V);
-  p.total = tokens * p.heads * p.units;
-  const int64_t blocks = (p.total + 255) / 256;
-  GPT_CHECK_SHAPE(blocks < (1LL << 31), "gpt_paged_kv_append: too many elements for one call");
-  launch_pdl(paged_append_kernel<T, V>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Append p) {
+  pdl_wait();
+  pdl_trigger();
+  const int id = (int)blockIdx.x * kAppendThreads + threadIdx.x;
+  if (id >= p.total) return;
+  for (int b = blockIdx.y; b < p.B; b += gridDim.y) append_one<T, V>(p, b, id);
+}
+
+template <typename T, int V>
+static int launch_append(Append p, int64_t heads, cudaStream_t st) {
+  const int64_t units = (p.D + 2 * V - 1) / (2 * V), total = p.T * heads * units;
+  GPT_CHECK_SHAPE(total < (1LL << 31) - kAppendThreads, "gpt_paged_kv_append: too many elements of one sequence for one call");
+  p.total = (int)total;
+  p.by_heads = FastDiv(heads);
+  p.by_units = FastDiv(units);
+  p.by_page = FastDiv(p.page);
+  const unsigned blocks = (unsigned)((total + kAppendThreads - 1) / kAppendThreads);
+  launch_pdl(paged_append_kernel<T, V>, dim3(blocks, (unsigned)(p.B < 65535 ? p.B : 65535)), dim3(kAppendThreads), 0, st, p);
   return launch_status("paged_kv_append");
 }
 
