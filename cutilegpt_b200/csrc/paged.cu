@@ -81,14 +81,19 @@ static void plan_launch(Kernel kernel, int64_t rows, int64_t items, int64_t keys
 }
 
 // The plan for the best kernel allowed.
-static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, Kernel best) {
+static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, int dtype, Kernel best) {
   int sms = device_sm_count();
   if (sms <= 0) sms = 148;
   Plan pl = {};
   const int64_t groups = kv->n_groups, per = groups > 0 ? kv->batch / groups : kv->batch;
   const int64_t rows = T * (H / kv->kv_heads), own_keys = kv->max_pages * kv->page_size;
   const int64_t pre_keys = groups > 0 ? kv->max_prefix_pages * kv->page_size : 0;
-  pl.shared = groups > 0 && per > 1 && (best != kTc || rows < kOwnTile);
+  // A prefix that is cheap to read for every sequence anew (from L2, by the CTAs that run anyway) saves a launch:
+  // 4 samples behind 96 positions, 12 heads: 14 us a call with a launch of its own, 11 without.
+  const int64_t size = dtype == GPT_F32 ? 4 : 2;
+  const bool cheap = rows <= kFewRows && pre_keys <= 256 &&
+                     kv->batch * kv->kv_heads * pre_keys * 2 * kv->head_dim * size <= (8 << 20);
+  pl.shared = groups > 0 && per > 1 && !cheap && (best != kTc || rows < kOwnTile);
   pl.pre = best;
   pl.own = best == kTc && rows <= kFewRows ? kRows : best;
   if (pl.shared) plan_launch(pl.pre, rows * per, groups * kv->kv_heads, pre_keys, sms, &pl.pre_splits, &pl.pre_two, &pl.n_pre);
@@ -101,6 +106,16 @@ static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, Kernel best)
   pl.acc_floats = (parts * kv->head_dim + 3) / 4 * 4;
   pl.bytes = (pl.acc_floats + 2 * parts) * (int64_t)sizeof(float);
   return pl;
+}
+
+// The largest workspace over the kernels that the alignment of q and out may ask for.
+static int64_t workspace_bytes(int64_t T, int64_t H, const gpt_paged_kv* kv, int dtype) {
+  int64_t most = 0;
+  for (int k = kSimt; k <= (dtype == GPT_BF16 ? kTc : kRows); ++k) {
+    const int64_t n = make_plan(T, H, kv, dtype, (Kernel)k).bytes;
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 template <typename T>
@@ -231,13 +246,7 @@ int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H, const g
   if (gpt::paged::check_kv(kv, "gpt_attention_shared_prefix_workspace_size") || (dtype != GPT_F32 && dtype != GPT_BF16) ||
       T <= 0 || H <= 0 || H % kv->kv_heads || kv->batch == 0)
     return 0;
-  // the largest over the kernels that the alignment of q and out may ask for
-  int64_t most = 0;
-  for (int k = gpt::paged::kSimt; k <= (dtype == GPT_BF16 ? gpt::paged::kTc : gpt::paged::kRows); ++k) {
-    const int64_t n = gpt::paged::make_plan(T, H, kv, (gpt::paged::Kernel)k).bytes;
-    most = n > most ? n : most;
-  }
-  return most;
+  return gpt::paged::workspace_bytes(T, H, kv, dtype);
 }
 
 int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* out, const int64_t* out_strides, int64_t T,
@@ -299,10 +308,11 @@ int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* o
   const gpt::paged::Kernel best = dtype == GPT_BF16 && gpt::paged::tc_eligible(p)              ? gpt::paged::kTc
                                   : gpt::paged::rows_eligible(p, dtype == GPT_BF16 ? 2 : 4) ? gpt::paged::kRows
                                                                                             : gpt::paged::kSimt;
-  const gpt::paged::Plan pl = gpt::paged::make_plan(T, H, kv, best);
-  GPT_CHECK_ARG(pl.bytes == 0 || (workspace && workspace_bytes >= pl.bytes),
-                "%s: workspace of %lld bytes required", what, (long long)pl.bytes);
-  GPT_CHECK_ALIGN(pl.bytes == 0 || gpt::aligned(workspace, 16), "%s: workspace needs 16-byte alignment", what);
+  const gpt::paged::Plan pl = gpt::paged::make_plan(T, H, kv, dtype, best);
+  const int64_t need = gpt::paged::workspace_bytes(T, H, kv, dtype);
+  GPT_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace of %lld bytes required", what,
+                (long long)need);
+  GPT_CHECK_ALIGN(need == 0 || gpt::aligned(workspace, 16), "%s: workspace needs 16-byte alignment", what);
   p.acc = (float*)workspace;
   p.ml = (float2*)((float*)workspace + pl.acc_floats);
   cudaStream_t st = (cudaStream_t)stream;

@@ -11,7 +11,6 @@ with the position rotation on the way where a model has one;
 from __future__ import annotations
 
 import ctypes
-import math
 
 import torch
 
@@ -116,8 +115,7 @@ class PagedKV:
 
 def _rows(t, name: str, kv: PagedKV, heads: int | None, tokens: int | None) -> torch.Tensor:
     """A (batch, heads, tokens, head_dim) tensor of the cache's type and device, head_dim contiguous."""
-    if not isinstance(t, torch.Tensor):
-        t = as_cuda(t, name)
+    t = as_cuda(t, name)
     shape = t.shape
     if (len(shape) != 4 or shape[0] != kv.batch or shape[3] != kv.head_dim or (heads is not None and shape[1] != heads)
             or (tokens is not None and shape[2] != tokens)):
@@ -128,6 +126,12 @@ def _rows(t, name: str, kv: PagedKV, heads: int | None, tokens: int | None) -> t
     return t if t.stride(3) == 1 or shape[3] == 1 else t.contiguous()
 
 
+def _out_rows(t, name: str, kv: PagedKV, heads: int, tokens: int) -> torch.Tensor:
+    if _rows(t, name, kv, heads, tokens) is not t:
+        raise ValueError(f"{name}: head_dim must be contiguous")
+    return t
+
+
 def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool = False, q_out=None):
     """Keys and values of new tokens into the cache; returns the queries, rotated where cos_sin is given.
 
@@ -136,7 +140,8 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
     to own position seq_lens[b] - tokens + t; a negative one is padding and is skipped. cos_sin
     float32 [n_pos, rot]: cosines, then sines, of the rot / 2 angles of each position; the first rot values of
     every query and key head are turned, in pairs (j, j + rot / 2) or, interleaved, (2j, 2j + 1), by the
-    position counted from the start of the prefix. q_out may be q itself.
+    position counted from the start of the prefix. q_out may be q itself; without cos_sin q is returned
+    as it is and may be None.
     """
     k = _rows(k, "k", kv, kv.n_kv_head, None)
     tokens = k.shape[2]
@@ -147,16 +152,15 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
         ops.paged_kv_append(None, k, v, None, kv)
         return q
     q = _rows(q, "q", kv, None, tokens)
-    cos_sin = as_cuda(cos_sin, "cos_sin")
-    if (cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous() or cos_sin.shape[0] == 0
-            or cos_sin.shape[1] % 2 or not 0 < cos_sin.shape[1] <= kv.head_dim or cos_sin.device != kv.device):
+    table = cos_sin.shape if isinstance(cos_sin, torch.Tensor) else ()
+    if (len(table) != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or table[0] == 0 or table[1] % 2
+            or not 0 < table[1] <= kv.head_dim or cos_sin.device != kv.device):
         raise ValueError(f"cos_sin: expected a contiguous float32 [n_pos, rot] table with even rot <= {kv.head_dim} on "
-                         f"{kv.device}, got {cos_sin.dtype} {tuple(cos_sin.shape)} on {cos_sin.device}")
+                         f"{kv.device}, got {getattr(cos_sin, 'dtype', type(cos_sin))} {tuple(table)}")
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        if _rows(q_out, "q_out", kv, q.shape[1], tokens) is not q_out:
-            raise ValueError("q_out: head_dim must be contiguous")
+        _out_rows(q_out, "q_out", kv, q.shape[1], tokens)
     ops.paged_kv_append(q, k, v, q_out, kv, cos_sin, interleaved)
     return q_out
 
@@ -168,15 +172,15 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
     h // (n_head // n_kv_head)); token t of sequence b sees the prefix and its own positions 0 ..
     seq_lens[b] - tokens + t, and gives zeros where that is negative (padding, idle sequences). The prefix
     is read once for all sequences of its group. scale is 1/√head_dim by default. A new contiguous tensor is
-    returned unless `out` (any strides, contiguous head_dim) is given; `workspace` (uint8,
+    returned unless `out` (any strides, contiguous head_dim, not q's memory) is given; `workspace` (uint8,
     kv.workspace_bytes(n_head, tokens)) is allocated unless given.
     """
     q = _rows(q, "q", kv, None, None)
-    heads, tokens = q.shape[1], q.shape[2]
+    _, heads, tokens, dim = q.shape
     if heads == 0 or heads % kv.n_kv_head:
         raise ValueError(f"shared_prefix_attention: {heads} heads are no multiple of {kv.n_kv_head} key heads")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    elif _rows(out, "out", kv, heads, tokens) is not out:
-        raise ValueError("out: head_dim must be contiguous")
-    return ops.shared_prefix_attention(q, kv, out, 1.0 / math.sqrt(kv.head_dim) if scale is None else scale, workspace)
+    else:
+        _out_rows(out, "out", kv, heads, tokens)
+    return ops.shared_prefix_attention(q, kv, out, dim ** -0.5 if scale is None else scale, workspace)

@@ -426,3 +426,38 @@ def test_refusals():
         with pytest.raises(ValueError):
             cg.cutile_paged_kv_append(*args)
     assert L.device_error() == 0
+
+
+def test_workspace_refusals():
+    kv, q = make(BF, 4, 1, 1, 4, 2, 64, 16, [900], [3, 4, 5, 6])
+    need = kv.workspace_bytes(4, 1)
+    assert need > 0
+    for ws in (torch.empty(need - 1, dtype=torch.uint8, device="cuda"), torch.empty(need, dtype=torch.uint8),
+               torch.empty(need + 16, dtype=torch.uint8, device="cuda")[3:]):
+        with pytest.raises(ValueError):
+            cg.cutile_shared_prefix_attention(q, kv, workspace=ws)
+    check_attention(q, kv, workspace=torch.empty(need, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype,interleaved,rot", [(BF, False, 128), (BF, True, 64), (F32, False, 64), (BF, False, 0)])
+def test_append_many_tokens(dtype, interleaved, rot):
+    """Prompts long enough for the variant that gives a thread two pairs of vectors."""
+    B, T, H, K, D, page = 2, 2100, 24, 8, 128, 64
+    n = -(-T // page)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages = torch.zeros(2, B * n, K, page, D, dtype=dtype, device="cuda")
+    order = torch.randperm(B * n, generator=g, device="cuda").int().view(B, n)
+    kv = cg.PagedKV(pages[0], pages[1], order, torch.full((B,), T, dtype=torch.int32, device="cuda"))
+    x = torch.randn(B, T, H + 2 * K, D, generator=g, device="cuda").to(dtype)
+    q, k, v = (y.transpose(1, 2) for y in x.split([H, K, K], dim=2))
+    table = torch.randn(T, rot, generator=g, device="cuda") if rot else None
+    got = cg.cutile_paged_kv_append(q, k, v, kv, table, interleaved)
+    in_order = [p[order.long()].transpose(1, 2).reshape(B, K, n * page, D)[:, :, :T] for p in pages]
+    assert torch.equal(in_order[1], v)
+    u = U[dtype]
+    for have, src in ((got, q), (in_order[0], k)):
+        if rot:
+            y, m = turned(src, table, rot, interleaved)
+            assert ((have.double() - y).abs() <= (4 * 2.0 ** -24 * m + u * y.abs()) * (m > 0)).all()
+        else:
+            assert torch.equal(have, src)
