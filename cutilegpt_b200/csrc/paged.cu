@@ -47,6 +47,7 @@ struct Plan {
   Kernel pre, own;         // kernels of the two launches (own: of the only one without `shared`)
   int pre_splits, pre_two, own_splits, own_two;
   int n_pre, n_own;        // slots of partial results; n_own = 0: the own launch writes out
+  int beside;              // the own launch runs beside the prefix launch and does not wait for it
   int64_t acc_floats;      // of the workspace: the accumulators, then the rows' (m, l)
   int64_t bytes;           // workspace
 };
@@ -99,9 +100,29 @@ static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, int dtype, K
   if (pl.shared) plan_launch(pl.pre, rows * per, groups * kv->kv_heads, pre_keys, sms, &pl.pre_splits, &pl.pre_two, &pl.n_pre);
   plan_launch(pl.own, rows, kv->batch * kv->kv_heads, own_keys + (pl.shared ? 0 : pre_keys), sms, &pl.own_splits, &pl.own_two,
               &pl.n_own);
+  if (pl.shared && pl.pre == kTc && pl.own == kRows) {
+    // A long prefix keeps the tensor cores busy, long own parts HBM: run beside each other they share the time. The
+    // prefix gets n of the SMs (one CTA each), the own launch fills the others at once and the prefix's when they
+    // end. Both times are estimated on the whole GPU, in us: pair of tiles 2.3 (D = 128) or 1.5, own keys (half of the
+    // table's positions) at 5500 GB/s, or at 55 GB/s for each SM where fewer read; both end together with
+    // sms pre / n = 100 own / (sms - n). B200, 128 sequences behind 64k positions, up to 4k own: 348 us one after
+    // the other, 322 beside; 67 sequences behind 8k, up to 1k own (pre = 11 us): 54 and 53, so not for short ones.
+    const int64_t blocks = groups * kv->kv_heads * ((rows * per + (pl.pre_two ? 255 : 127)) / (pl.pre_two ? 256 : 128));
+    const double passes = (double)blocks * ((pre_keys + 127) / 128) / (pl.pre_two ? 1 : 2);
+    const double pre = passes * (kv->head_dim > 64 ? 2.3 : 1.5) / sms;
+    const double own = (double)kv->batch * kv->kv_heads * own_keys * 4 * kv->head_dim / 2 / 5.5e6;
+    if (pre > 20 && own > 20) {
+      const double n = (double)sms * sms * pre / (100 * own + sms * pre);
+      const int splits = (int)(n / blocks + 0.999);
+      if (splits < pl.pre_splits) {
+        pl.pre_splits = pl.n_pre = splits < 1 ? 1 : splits;
+        pl.beside = 1;
+      }
+    }
+  }
   // one share: the kernel joins the prefix's slots itself and writes out (the tcgen05 kernel: where there are none;
   // the few-row kernel: as many as it has room for)
-  if (pl.n_own == 1 && (pl.own == kTc ? pl.n_pre == 0 : pl.own == kRows ? pl.n_pre <= kMaxSlots : true)) pl.n_own = 0;
+  if (pl.n_own == 1 && !pl.beside && (pl.own == kTc ? pl.n_pre == 0 : pl.own == kRows ? pl.n_pre <= kMaxSlots : true)) pl.n_own = 0;
   const int64_t parts = (int64_t)(pl.n_pre + pl.n_own) * kv->batch * T * H;
   pl.acc_floats = (parts * kv->head_dim + 3) / 4 * 4;
   pl.bytes = (pl.acc_floats + 2 * parts) * (int64_t)sizeof(float);
@@ -159,7 +180,7 @@ static int run(Attn& p, const Plan& pl, cudaStream_t st) {
   p.n_own = pl.n_own;
   int s = GPT_OK;
   if (pl.shared) s = launch<T>(pl.pre, p, kPrefix, pl.pre_splits, pl.pre_two, 0, 0, 0, st);
-  if (!s) s = launch<T>(pl.own, p, pl.shared ? kOwn : kAll, pl.own_splits, pl.own_two, pl.n_pre, pl.n_own == 0, pl.shared, st);
+  if (!s) s = launch<T>(pl.own, p, pl.shared ? kOwn : kAll, pl.own_splits, pl.own_two, pl.n_pre, pl.n_own == 0, pl.shared ? 1 + pl.beside : 0, st);
   if (!s && pl.n_own > 0) s = launch_join<T>(p, st);
   return s;
 }

@@ -15,8 +15,11 @@
 //
 // bf16: m16n8k16. P is rounded to bf16 for its product with V, its sum is taken before.
 // fp32: m16n8k8 on TF32 parts. A value x is hi + lo, hi = x to 11 bits, lo = (x - hi) to
-// 11 bits: x is met to 2^-22, and hi hi + hi lo + lo hi leaves out 2^-22 of a product. The order of a
-// contraction is free, so a lane's operands are those that one 16-byte read gives it.
+// 11 bits: x is met to 2^-22, and hi hi + hi lo + lo hi leaves out 2^-22 of a product. The tensor cores
+// cut sums off towards zero, so a product chain is short (16 elements of a score, a step's keys of
+// the output) and is added to the running sum by a rounding add (13 samples of 1003 + 77 positions against
+// 64 bits: 1.2e-6 off with chains through, 4.3e-7 so). The order of a contraction is free, so a lane's operands are
+// those that one 16-byte read gives it.
 #include "paged.cuh"
 
 namespace gpt {
@@ -119,7 +122,8 @@ __device__ __forceinline__ void store4(T* dst, float4 v) {
 }
 
 struct RowsArgs {
-  int phase, splits, slot0, direct, early;
+  int phase, splits, slot0, direct;
+  int early;                // behind this call's prefix launch: 1 waits for it before the end, 2 runs beside it
   int two_warps;            // CTAs of two warps, not four
   FastDiv by_splits, by_blocks;
 };
@@ -280,10 +284,12 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
         }
 #pragma unroll
         for (int i = 0; i < KS / 8; ++i) {
-          float kv[4];
+          float kv[4], part[4] = {0.f, 0.f, 0.f, 0.f};
           lds128(sk + swz<T, DP>(i * 8 + lane / 4, k * 4 + quad), kv);
-          mma_split(sc[i], ah[0], al[0], kv[0], kv[1]);
-          mma_split(sc[i], ah[1], al[1], kv[2], kv[3]);
+          mma_split(part, ah[0], al[0], kv[0], kv[1]);
+          mma_split(part, ah[1], al[1], kv[2], kv[3]);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) sc[i][u] += part[u];
         }
       }
     } else {
@@ -341,21 +347,29 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
         l[k >> 1] += sc[i][k];
       }
     if constexpr (kWide) {
+      uint32_t ah[KS / 8][4], al[KS / 8][4];
 #pragma unroll
       for (int i = 0; i < KS / 8; ++i) {   // contraction index quad is key 2 quad, quad + 4 is key 2 quad + 1
-        uint32_t ah[4], al[4];
-        split_tf32(sc[i][0], ah[0], al[0]);
-        split_tf32(sc[i][2], ah[1], al[1]);
-        split_tf32(sc[i][1], ah[2], al[2]);
-        split_tf32(sc[i][3], ah[3], al[3]);
+        split_tf32(sc[i][0], ah[i][0], al[i][0]);
+        split_tf32(sc[i][2], ah[i][1], al[i][1]);
+        split_tf32(sc[i][1], ah[i][2], al[i][2]);
+        split_tf32(sc[i][3], ah[i][3], al[i][3]);
+      }
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {   // column index g of product u is element 32 d + 4 g + u
+      for (int d = 0; d < DP / 32; ++d) {   // column index g of product u is element 32 d + 4 g + u
+        float part[4][4] = {};
+#pragma unroll
+        for (int i = 0; i < KS / 8; ++i) {
           float v0[4], v1[4];
           lds128(sv + swz<T, DP>(i * 8 + 2 * quad, d * 8 + lane / 4), v0);
           lds128(sv + swz<T, DP>(i * 8 + 2 * quad + 1, d * 8 + lane / 4), v1);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mma_split(o[4 * d + u], ah, al, v0[u], v1[u]);
+          for (int u = 0; u < 4; ++u) mma_split(part[u], ah[i], al[i], v0[u], v1[u]);
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[4 * d + u][k] += part[u][k];
       }
     } else {
 #pragma unroll
@@ -406,7 +420,9 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     }
   }
   __syncthreads();
-  if (a.early) pdl_wait();   // the prefix launch's partial results; its end, for whatever comes after this launch
+  // the prefix launch's partial results; its end, which the launch that joins must not come before: for
+  // that one CTA's wait is enough, and the others make room for the next
+  if (a.early == 1 || (a.early == 2 && blockIdx.x == 0)) pdl_wait();
   // A row's parts: the prefix's slots and the CTA's warps, in that order. Everything that comes from global
   // memory is asked for at once: the slots' (m, l) of all rows, by all threads, and the first slots'
   // columns of the thread's first item.
