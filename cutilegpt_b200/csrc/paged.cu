@@ -14,20 +14,20 @@ static int check_kv(const gpt_paged_kv* kv, const char* what) {
                       kv->head_dim > 0 && kv->head_dim <= 256,
                   "%s: bad sizes batch=%lld kv_heads=%lld head_dim=%lld (1..256)", what, (long long)kv->batch,
                   (long long)kv->kv_heads, (long long)kv->head_dim);
-  GPT_CHECK_SHAPE(kv->n_pages > 0 && kv->n_pages < (1LL << 31) && kv->page_size > 0 && kv->page_size < (1LL << 30),
+  GPT_CHECK_SHAPE(kv->n_pages > 0 && kv->n_pages < (1LL << 31) && kv->page_size > 0 && kv->page_size < (1LL << 29),
                   "%s: bad sizes n_pages=%lld page_size=%lld", what, (long long)kv->n_pages, (long long)kv->page_size);
   GPT_CHECK_SHAPE(kv->page_stride >= 0 && kv->head_stride >= 0 && kv->slot_stride >= 0,
                   "%s: negative cache stride", what);
-  GPT_CHECK_SHAPE(kv->max_pages > 0 && kv->max_pages <= (1LL << 30) / kv->page_size &&
+  GPT_CHECK_SHAPE(kv->max_pages > 0 && kv->max_pages <= (1LL << 29) / kv->page_size &&
                       kv->ld_page_table >= kv->max_pages,
-                  "%s: page_table rows list %lld pages (row stride %lld) of %lld positions; a row lists 1 to 2^30 positions",
+                  "%s: page_table rows list %lld pages (row stride %lld) of %lld positions; a row lists 1 to 2^29 positions",
                   what, (long long)kv->max_pages, (long long)kv->ld_page_table, (long long)kv->page_size);
   GPT_CHECK_SHAPE(kv->n_groups >= 0 && (kv->n_groups == 0 || kv->batch % kv->n_groups == 0),
                   "%s: n_groups=%lld does not divide batch=%lld", what, (long long)kv->n_groups, (long long)kv->batch);
   if (kv->n_groups > 0)
-    GPT_CHECK_SHAPE(kv->max_prefix_pages > 0 && kv->max_prefix_pages <= (1LL << 30) / kv->page_size &&
+    GPT_CHECK_SHAPE(kv->max_prefix_pages > 0 && kv->max_prefix_pages <= (1LL << 29) / kv->page_size &&
                         kv->ld_prefix_table >= kv->max_prefix_pages,
-                    "%s: prefix_table rows list %lld pages (row stride %lld) of %lld positions; a row lists 1 to 2^30 positions",
+                    "%s: prefix_table rows list %lld pages (row stride %lld) of %lld positions; a row lists 1 to 2^29 positions",
                     what, (long long)kv->max_prefix_pages, (long long)kv->ld_prefix_table, (long long)kv->page_size);
   return GPT_OK;
 }
@@ -40,6 +40,9 @@ static int check_kv_pointers(const gpt_paged_kv* kv, const char* what) {
 
 // The kernels of an attention call, in the order of preference for the calls that they can serve.
 enum Kernel { kSimt = 0, kRows = 1, kTc = 2 };
+
+// The stride of a dimension of one element says nothing: 8 keeps every alignment.
+static int64_t used_stride(int64_t size, int64_t stride) { return size == 1 ? 8 : stride; }
 
 // How an attention call runs.
 struct Plan {
@@ -289,17 +292,18 @@ int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides, void* o
   gpt::paged::Attn p = {};
   p.q = q;
   p.out = out;
-  p.q_b = q_strides[0];
-  p.q_h = q_strides[1];
-  p.q_t = q_strides[2];
-  p.o_b = out_strides[0];
-  p.o_h = out_strides[1];
-  p.o_t = out_strides[2];
+  using gpt::paged::used_stride;
+  p.q_b = used_stride(kv->batch, q_strides[0]);
+  p.q_h = used_stride(H, q_strides[1]);
+  p.q_t = used_stride(T, q_strides[2]);
+  p.o_b = used_stride(kv->batch, out_strides[0]);
+  p.o_h = used_stride(H, out_strides[1]);
+  p.o_t = used_stride(T, out_strides[2]);
   p.k = kv->k_pages;
   p.v = kv->v_pages;
-  p.page_stride = kv->page_stride;
-  p.head_stride = kv->head_stride;
-  p.slot_stride = kv->slot_stride;
+  p.page_stride = used_stride(kv->n_pages, kv->page_stride);
+  p.head_stride = used_stride(kv->kv_heads, kv->head_stride);
+  p.slot_stride = used_stride(kv->page_size, kv->slot_stride);
   p.n_pages = (int)kv->n_pages;
   p.page = (int)kv->page_size;
   p.table = kv->page_table;

@@ -155,26 +155,61 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Attn 
   }
 }
 
-// out of all partial slots, one warp per row.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const Attn p) {
-  constexpr int NC = kSimtMaxD / 32;
+// out of all partial slots: `groups` teams of D / 4 threads a row (four columns a thread; D threads, one column
+// each, where D is no multiple of 4), team g takes slots g, g + groups, ..., eight loads at a time, and the teams are
+// joined in order through shared memory.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Attn p, int groups, int rows_cta) {
+  struct alignas(4 * V) Cols {
+    float c[V];
+  };
+  __shared__ float2 sm_ml[kJoinThreads];
+  __shared__ Cols sm_acc[kJoinThreads];
   pdl_wait();
   pdl_trigger();
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)p.B * p.T * p.H) return;
-  const int lane = threadIdx.x & 31;
+  const int team = p.D / V, who = threadIdx.x / team, d = (threadIdx.x - who * team) * V;
+  const int64_t rows = (int64_t)p.B * p.T * p.H, row = (int64_t)blockIdx.x * rows_cta + who / groups;
+  const int group = who % groups, n = p.n_pre + p.n_own;
+  const bool mine = who < rows_cta * groups && row < rows;
+  float m = -INFINITY, l = 0.f;
+  Cols acc = {};
+  auto add = [&](float2 ml, const Cols& v) {   // a slot without keys has l = 0 and was not written
+    if (ml.y == 0.f) return;
+    const float to = fmaxf(m, ml.x), a = l == 0.f ? 0.f : exp2f(m - to), b = exp2f(ml.x - to);
+    m = to;
+    l = l * a + ml.y * b;
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc.c[i] = acc.c[i] * a + v.c[i] * b;
+  };
+  for (int s0 = group; mine && s0 < n; s0 += 8 * groups) {
+    float2 ml[8];
+    Cols v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int s = s0 + i * groups;
+      ml[i] = make_float2(0.f, 0.f);
+      if (s >= n) continue;
+      ml[i] = p.ml[s * rows + row];
+      v[i] = *reinterpret_cast<const Cols*>(p.acc + (s * rows + row) * p.D + d);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) add(ml[i], v[i]);
+  }
+  if (groups > 1) {
+    sm_ml[threadIdx.x] = make_float2(m, l);
+    sm_acc[threadIdx.x] = acc;
+    __syncthreads();
+    if (group != 0) return;
+    for (int g = 1; mine && g < groups; ++g) add(sm_ml[threadIdx.x + g * team], sm_acc[threadIdx.x + g * team]);
+  }
+  if (!mine || group != 0) return;
   const int h = (int)(row % p.H), t = (int)(row / p.H % p.T), b = (int)(row / p.H / p.T);
-  float m = -INFINITY, l = 0.f, acc[NC];
+  const float inv = l == 0.f || last_key(p, b, t) < 0 ? 0.f : 1.f / l;   // 0: padding
+  T* out = (T*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d;
 #pragma unroll
-  for (int k = 0; k < NC; ++k) acc[k] = 0.f;
-  const bool padding = last_key(p, b, t) < 0;
-  if (!padding) join_slots<NC>(p, 0, p.n_pre + p.n_own, row, lane, m, l, acc);
-  const float inv = 1.f / l;
-  T* out = (T*)p.out + b * p.o_b + h * p.o_h + t * p.o_t;
-#pragma unroll
-  for (int k = 0; k < NC; ++k)
-    if (lane + 32 * k < p.D) out[lane + 32 * k] = Tr<T>::from_f(padding ? 0.f : acc[k] * inv);
+  for (int i = 0; i < V; ++i) out[i] = Tr<T>::from_f(inv == 0.f ? 0.f : acc.c[i] * inv);
 }
 
 template <typename T, int RB>
@@ -200,11 +235,22 @@ static int launch_simt(const Attn& p, int phase, int splits, int slot0, int dire
                    : launch_simt_rb<T, 16>(p, phase, splits, slot0, direct, st);
 }
 
+template <typename T, int V>
+static int launch_join_v(const Attn& p, cudaStream_t st) {
+  const int team = p.D / V, teams = kJoinThreads / team, n = p.n_pre + p.n_own;
+  // teams for a row: as many as the slots keep busy with eight loads, so that many slots cost few rounds
+  int groups = 1;
+  while (groups * 8 < n && groups * 2 <= teams) groups *= 2;
+  const int rows_cta = teams / groups;
+  const int64_t rows = (int64_t)p.B * p.T * p.H;
+  launch_pdl(paged_join_kernel<T, V>, dim3((unsigned)((rows + rows_cta - 1) / rows_cta)), dim3(kJoinThreads), 0, st, p, groups,
+             rows_cta);
+  return launch_status("paged_join");
+}
+
 template <typename T>
 static int launch_join(const Attn& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.B * p.T * p.H;
-  launch_pdl(paged_join_kernel<T>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, p);
-  return launch_status("paged_join");
+  return p.D % 4 == 0 ? launch_join_v<T, 4>(p, st) : launch_join_v<T, 1>(p, st);
 }
 
 }  // namespace paged

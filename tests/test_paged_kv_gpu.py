@@ -128,6 +128,13 @@ ATTENTION = [
     (BF, 70, 1, 2, 8, 2, 128, 16, [300], [2 + i for i in range(70)]),
     (BF, 1, 1, 1, 1, 1, 64, 16, [1], [1]),
     (BF, 130, 1, 1, 2, 1, 128, 64, [1025], [(i * 5) % 9 for i in range(130)]),
+    (BF, 1, 0, 1, 2, 1, 128, 64, [], [9000]),                             # one sequence, dozens of shares of its keys
+    (F32, 1, 0, 1, 1, 1, 64, 32, [], [5001]),
+    (BF, 1, 0, 2, 3, 1, 7, 16, [], [3000]),
+    (BF, 8, 1, 1, 1, 1, 64, 128, [20000], [9, 3, 1, 4, 100, 2, 7, 8]),    # many shares of the prefix
+    (F32, 20, 1, 1, 4, 2, 32, 16, [700], [i % 7 for i in range(20)]),
+    (BF, 3, 1, 20, 8, 1, 64, 16, [333], [20, 47, 90]),                    # rows of a sequence fill no tile, prefix shared
+    (BF, 64, 1, 1, 32, 8, 128, 128, [33000], [(37 * i) % 2000 + 1 for i in range(64)]),   # prefix beside own parts
 ]
 
 
@@ -160,6 +167,15 @@ def test_attention_unaligned_views():
     out = torch.empty(q.numel() + 5, dtype=BF, device="cuda")[5:].view(3, 4, 1, 64)
     check_attention(odd, cg.PagedKV(*pages, kv.page_table, kv.seq_lens, kv.prefix_table, kv.prefix_lens), out=out)
     check_attention(q, kv, out=out)
+
+
+def test_attention_strides_of_single_dimensions():
+    """The stride of a dimension of size 1 is never used, whatever it says."""
+    kv, q = make(BF, 2, 1, 1, 4, 1, 64, 16, [40], [3, 17])
+    kp, vp = (torch.as_strided(x, x.shape, (x.stride(0), 3, x.stride(2), 1)) for x in (kv.k_pages, kv.v_pages))
+    odd = cg.PagedKV(kp, vp, kv.page_table, kv.seq_lens, kv.prefix_table, kv.prefix_lens)
+    q1 = torch.as_strided(q, q.shape, (q.stride(0), q.stride(1), 5, 1), q.storage_offset())
+    assert torch.equal(check_attention(q1, odd), cg.cutile_shared_prefix_attention(q, kv))
 
 
 def test_attention_peaked_and_huge_scores():
