@@ -98,7 +98,9 @@ static Plan make_plan(int64_t T, int64_t H, const gpt_paged_kv* kv, int dtype, K
   const bool cheap = rows <= kFewRows && pre_keys <= 256 &&
                      kv->batch * kv->kv_heads * pre_keys * 2 * kv->head_dim * size <= (8 << 20);
   pl.shared = groups > 0 && per > 1 && !cheap && (best != kTc || rows < kOwnTile);
-  pl.pre = best;
+  // Few rows in all fill no 128-row tile: 8 prompts with 8 samples each, 25 heads: 37 us with the tcgen05 kernel
+  // for the prefixes, 29 with the few-row one, whose CTAs run among the own launch's.
+  pl.pre = best == kTc && rows * per <= kFewRows ? kRows : best;
   pl.own = best == kTc && rows <= kFewRows ? kRows : best;
   if (pl.shared) plan_launch(pl.pre, rows * per, groups * kv->kv_heads, pre_keys, sms, &pl.pre_splits, &pl.pre_two, &pl.n_pre);
   plan_launch(pl.own, rows, kv->batch * kv->kv_heads, own_keys + (pl.shared ? 0 : pre_keys), sms, &pl.own_splits, &pl.own_two,
