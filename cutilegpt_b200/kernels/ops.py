@@ -200,28 +200,25 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     return out
 
 
-def _strides3(t: torch.Tensor | None):
-    return None if t is None else L.strides3(*t.stride()[:3])
-
-
-def _on_device(kv, fn, *args) -> int:
-    """fn(*args, stream) with the device of `kv` current (a launch goes to the current device)."""
-    index = kv.device.index
-    if index == torch.cuda.current_device():
-        return fn(*args, L.stream_ptr(kv.device))
-    with torch.cuda.device(index):
-        return fn(*args, L.stream_ptr(kv.device))
-
-
 def paged_kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: torch.Tensor | None, kv,
                     cos_sin: torch.Tensor | None = None, interleaved: bool = False) -> None:
     """k, v [B, K, T, D] views into the pages of `kv` (a PagedKV); with cos_sin [n_pos, rot] the keys
     and q [B, H, T, D] are rotated, q into q_out."""
-    n_pos, rot = cos_sin.shape if cos_sin is not None else (0, 0)
-    heads = q.shape[1] if q is not None else kv.n_kv_head
-    status = _on_device(kv, L.lib().gpt_paged_kv_append, _ptr(q), _strides3(q), k.data_ptr(), _strides3(k), v.data_ptr(),
-                        _strides3(v), _ptr(q_out), _strides3(q_out), k.shape[2], heads, kv._ref, _ptr(cos_sin), n_pos, rot,
-                        int(interleaved), kv._dtype_code)
+    if kv.device.index != torch.cuda.current_device():   # a launch goes to the current device
+        with torch.cuda.device(kv.device):
+            return paged_kv_append(q, k, v, q_out, kv, cos_sin, interleaved)
+    strides = L.strides3
+    if cos_sin is None:
+        status = L.lib().gpt_paged_kv_append(None, None, k.data_ptr(), strides(*k.stride()[:3]), v.data_ptr(),
+                                             strides(*v.stride()[:3]), None, None, k.shape[2], kv.n_kv_head, kv._ref, None, 0,
+                                             0, 0, kv._dtype_code, L.stream_ptr(kv.device))
+    else:
+        _, heads, tokens, _ = q.shape
+        n_pos, rot = cos_sin.shape
+        status = L.lib().gpt_paged_kv_append(q.data_ptr(), strides(*q.stride()[:3]), k.data_ptr(), strides(*k.stride()[:3]),
+                                             v.data_ptr(), strides(*v.stride()[:3]), q_out.data_ptr(),
+                                             strides(*q_out.stride()[:3]), tokens, heads, kv._ref, cos_sin.data_ptr(), n_pos,
+                                             rot, 1 if interleaved else 0, kv._dtype_code, L.stream_ptr(kv.device))
     if status:
         L.check(status, "gpt_paged_kv_append")
 
@@ -230,6 +227,9 @@ def shared_prefix_attention(q: torch.Tensor, kv, out: torch.Tensor, scale: float
                             workspace: torch.Tensor | None = None) -> torch.Tensor:
     """q, out [B, H, T, D] views over the cache `kv` (a PagedKV). The workspace, kv.workspace_bytes(H, T)
     bytes of uint8, is allocated (on the current stream) when it is None."""
+    if kv.device.index != torch.cuda.current_device():
+        with torch.cuda.device(kv.device):
+            return shared_prefix_attention(q, kv, out, scale, workspace)
     _, H, T, _ = q.shape
     if workspace is None:
         have = kv.workspace_bytes(H, T)
@@ -239,8 +239,11 @@ def shared_prefix_attention(q: torch.Tensor, kv, out: torch.Tensor, scale: float
         raise ValueError("shared_prefix_attention: the workspace must be a contiguous tensor on the cache's device")
     else:
         have = workspace.numel() * workspace.element_size()
-    status = _on_device(kv, L.lib().gpt_attention_shared_prefix, q.data_ptr(), _strides3(q), out.data_ptr(), _strides3(out),
-                        T, H, kv._ref, scale, _ptr(workspace), have, kv._dtype_code)
+    strides = L.strides3
+    status = L.lib().gpt_attention_shared_prefix(q.data_ptr(), strides(*q.stride()[:3]), out.data_ptr(),
+                                                 strides(*out.stride()[:3]), T, H, kv._ref, scale,
+                                                 None if workspace is None else workspace.data_ptr(), have, kv._dtype_code,
+                                                 L.stream_ptr(kv.device))
     if status:
         L.check(status, "gpt_attention_shared_prefix")
     return out

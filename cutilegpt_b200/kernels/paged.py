@@ -115,15 +115,16 @@ class PagedKV:
 
 def _rows(t, name: str, kv: PagedKV, heads: int | None, tokens: int | None) -> torch.Tensor:
     """A (batch, heads, tokens, head_dim) tensor of the cache's type and device, head_dim contiguous."""
-    t = as_cuda(t, name)
+    if type(t) is not torch.Tensor:
+        t = as_cuda(t, name)
     shape = t.shape
-    if (len(shape) != 4 or shape[0] != kv.batch or shape[3] != kv.head_dim or (heads is not None and shape[1] != heads)
-            or (tokens is not None and shape[2] != tokens)):
+    b, h, n, d = shape if len(shape) == 4 else (-1, 0, 0, 0)
+    if b != kv.batch or d != kv.head_dim or (heads is not None and h != heads) or (tokens is not None and n != tokens):
         raise ValueError(f"{name}: expected ({kv.batch}, {'n_head' if heads is None else heads}, "
                          f"{'tokens' if tokens is None else tokens}, {kv.head_dim}), got {tuple(shape)}")
     if t.dtype != kv.dtype or t.device != kv.device:
         raise ValueError(f"{name}: {t.dtype} on {t.device}, but the cache holds {kv.dtype} on {kv.device}")
-    return t if t.stride(3) == 1 or shape[3] == 1 else t.contiguous()
+    return t if t.stride(3) == 1 or d == 1 else t.contiguous()
 
 
 def _out_rows(t, name: str, kv: PagedKV, heads: int, tokens: int) -> torch.Tensor:
