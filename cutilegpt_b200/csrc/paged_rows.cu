@@ -12,9 +12,9 @@
 // (mma.sync: 16 rows cannot fill the 128 rows of a tcgen05 tile; those run in paged_tc.cu).
 // No barrier stands between a warp's loads and its products; 12 to 16 warps of an
 // SM keep 96 to 128 KB in flight.
-// B200: own keys of 128 sequences, up to 4096 each, 8 key heads of 128 in bf16 (1.07 GB): 190 us = 5.6 TB/s; 67
-// sequences of up to 1024: 28 us = 4.8 TB/s. Below some 300 keys a CTA its fixed chain rules (length, page
-// table, first copies, join: about 5 us): 64 sequences of up to 256, 12 heads of 64: 8 us for 26 MB.
+// B200: 128 sequences of up to 4096 positions, 8 key heads of 128 in bf16 (1.08 GB): 174 us = 6.2 TB/s, 0.95 of a
+// measured copy; 67 of up to 1024: 36 us = 4.0 TB/s (the last CTAs alone). Below some 300 keys a CTA its fixed
+// chain rules (length, page table, first copies, join: about 5 us): 64 of up to 256, 12 heads of 64: 13.4 us.
 //
 // bf16: m16n8k16. P is rounded to bf16 for its product with V, its sum is taken before.
 // fp32: m16n8k8 on TF32 parts. A value x is hi + lo, hi = x to 11 bits, lo = (x - hi) to
@@ -36,7 +36,9 @@ struct Rows {
   static constexpr bool kWide = sizeof(T) == 4;
   static constexpr int kKeys = kWide ? (DP == 128 ? 8 : DP == 64 ? 16 : 32) : (DP >= 64 ? 16 : 1024 / DP);   // of a warp's step
   static constexpr int kTile = kKeys * DP * (int)sizeof(T);    // bytes of a step's keys
-  static constexpr int kRing = kTile > 2048 ? 2 : 3;           // steps of a warp's ring
+  // Steps of a warp's ring. Deeper ones cost resident CTAs: with four warps a fourth step pays (48 drafts of 5 tokens,
+  // D = 64: 31.5 -> 30.0 us), with two it does not (64 samples of 768 + 256 positions: 13.4 us, 18.7 with four steps).
+  static constexpr int kRing = kTile > 2048 ? 2 : W == 4 ? 4 : 3;
   static constexpr int kCtas = (kWide ? 8 : DP == 128 ? 12 : 16) / W;   // of an SM
   // Q fragments in shared memory, read at every step, where they would take too many registers
   static constexpr bool kQShared = kWide || DP == 128;
