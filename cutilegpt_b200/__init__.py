@@ -3,7 +3,9 @@
 Mirrors the reference package facade (cutile_gpt/__init__.py:41-129): the
 seven kernel operators, the model (CutileGPT, GPTConfig) and the Tile API,
 with hand-written CUDA kernels behind a C ABI (include/gpt_b200.h,
-libgpt_b200.so) instead of cuTile.
+libgpt_b200.so) instead of cuTile. Beside them, without a reference
+counterpart: a paged key/value cache (PagedKV, cutile_paged_kv_append,
+cutile_shared_prefix_attention; CutileGPT.generate_samples uses it).
 """
 __version__ = "0.1.0"
 
