@@ -121,5 +121,46 @@ struct Keys {
   }
 };
 
+// ---- infinities and NaN in values that not every row of a tile sees -----------
+// The tensor-core kernels give such a value the probability 0 for the rows that do not see it, and multiply:
+// 0 x inf would reach outputs it has no part in. They look through the value tiles at the causal edge (T > 1 only)
+// and, where one holds such a value, compute the CTA's rows again here, key by key.
+template <typename T>
+__device__ __forceinline__ bool non_finite(uint32_t w) {   // either bf16 of the pair, or the fp32
+  if constexpr (sizeof(T) == 2)
+    return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  else
+    return (w & 0x7f800000u) == 0x7f800000u;
+}
+template <typename T>
+__device__ __forceinline__ bool non_finite(uint4 v) {
+  return non_finite<T>(v.x) || non_finite<T>(v.y) || non_finite<T>(v.z) || non_finite<T>(v.w);
+}
+
+// Row `q` against keys j0 .. j1 - 1 by one warp: m, l and acc (columns lane + 32 c), D <= 128.
+template <typename T>
+__device__ __noinline__ void slow_row(const Attn& p, const Keys keys, int kh, const T* q, int j0, int j1, int lane, float& m,
+                                      float& l, float (&acc)[4]) {
+  float x[4];
+  m = -INFINITY;
+  l = 0.f;
+  for (int c = 0; c < 4; ++c) {
+    x[c] = lane + 32 * c < p.D ? Tr<T>::to_f(q[lane + 32 * c]) : 0.f;
+    acc[c] = 0.f;
+  }
+  for (int j = j0; j < j1; ++j) {
+    const int64_t off = keys.offset(p, j, kh);
+    float s = 0.f;
+    for (int c = 0; c < 4; ++c)
+      if (off >= 0 && lane + 32 * c < p.D) s = fmaf(x[c], Tr<T>::to_f(((const T*)p.k)[off + lane + 32 * c]), s);
+    s = warp_sum(s) * p.scale_log2;
+    const float to = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - to), e = to == -INFINITY ? 0.f : exp2f(s - to);
+    m = to;
+    l = l * a + e;
+    for (int c = 0; c < 4; ++c)
+      if (lane + 32 * c < p.D) acc[c] = acc[c] * a + (off < 0 ? 0.f : e * Tr<T>::to_f(((const T*)p.v)[off + lane + 32 * c]));
+  }
+}
+
 }  // namespace paged
 }  // namespace gpt

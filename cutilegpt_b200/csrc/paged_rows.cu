@@ -87,6 +87,11 @@ __device__ __forceinline__ void lds128(uint32_t addr, float (&r)[4]) {
                : "r"(addr)
                : "memory");
 }
+__device__ __forceinline__ uint4 lds_u4(uint32_t addr) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(addr) : "memory");
+  return r;
+}
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -133,8 +138,10 @@ struct RowsArgs {
   FastDiv by_splits, by_blocks;
 };
 
-template <typename T, int DP, int W>
-__global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_kernel(const Attn p, const RowsArgs a) {
+// kEdge: several tokens a sequence and own keys, so that rows of the tile see different keys.
+template <typename T, int DP, int W, bool kEdge>
+__global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_kernel(const __grid_constant__ Attn p,
+                                                                                     const RowsArgs a) {
   using C = Rows<T, DP, W>;
   constexpr bool kWide = C::kWide;
   constexpr int KS = C::kKeys, kPer = 16 / (int)sizeof(T), kChunks = DP / kPer, kLoads = KS * kChunks / 32;
@@ -266,6 +273,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
   for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
     for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+  const bool edge = least < j1;     // some rows see keys of this share that others do not
+  bool odd = false;
   for (int s = 0; s < steps; ++s) {
     cp_wait<kRing - 2>();
     __syncwarp();
@@ -312,6 +321,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
       }
     }
     if (j + KS > least) {   // keys that some row does not see
+      if (kEdge && edge)    // see slow_row
+        for (int i = lane; i < kTile / 16; i += 32) odd |= non_finite<T>(lds_u4(sv + i * 16));
 #pragma unroll
       for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
@@ -402,7 +413,11 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
 
   // the warps' results joined through shared memory, where the rings were
   cp_wait<0>();
-  __syncthreads();
+  bool again = false;
+  if (kEdge)
+    again = __syncthreads_or(odd);
+  else
+    __syncthreads();
   float* sm_o = reinterpret_cast<float*>(rows_smem_dyn + C::kQ);         // [warp][16][DP]
   float2* sm_ml = reinterpret_cast<float2*>(sm_o + W * kRowTile * DP);   // [warp][16]
   float2* sm_w = sm_ml + W * kRowTile;                                   // [16][kMaxSlots]
@@ -425,6 +440,21 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     }
   }
   __syncthreads();
+  if (kEdge && again) {
+    for (int rl = warp; rl < kRowTile; rl += W) {
+      float rm = -INFINITY, rls = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+      if (r0 + rl < rows) {
+        const Row at(p, b0, kh, r0 + rl);
+        const int last = keys.n_own - p.T + at.t;
+        slow_row<T>(p, keys, kh, (const T*)p.q + at.b * p.q_b + at.h * p.q_h + at.t * p.q_t, j0,
+                    last < 0 ? j0 : min(j1, keys.n_pre + last + 1), lane, rm, rls, acc);
+      }
+      if (lane < W) sm_ml[lane * kRowTile + rl] = lane == 0 ? make_float2(rm, rls) : make_float2(-INFINITY, 0.f);
+      for (int c = 0; c < 4; ++c)
+        if (lane + 32 * c < p.D) sm_o[rl * DP + lane + 32 * c] = acc[c];
+    }
+    __syncthreads();
+  }
   // the prefix launch's partial results; its end, which the launch that joins must not come before: for
   // that one CTA's wait is enough, and the others make room for the next
   if (a.early == 1 || (a.early == 2 && blockIdx.x == 0)) pdl_wait();
@@ -502,7 +532,7 @@ static bool rows_eligible(const Attn& p, int size) {
   return true;
 }
 
-template <typename T, int DP, int W>
+template <typename T, int DP, int W, bool kEdge>
 static int launch_rows_w(const Attn& p, RowsArgs a, cudaStream_t st) {
   using C = Rows<T, DP, W>;
   static bool done[64] = {false};
@@ -512,7 +542,7 @@ static int launch_rows_w(const Attn& p, RowsArgs a, cudaStream_t st) {
   {
     std::lock_guard<std::mutex> g(mu);
     if (dev >= 0 && dev < 64 && !done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, DP, W>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+      cudaError_t e = cudaFuncSetAttribute(paged_rows_kernel<T, DP, W, kEdge>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       done[dev] = true;
     }
@@ -523,13 +553,15 @@ static int launch_rows_w(const Attn& p, RowsArgs a, cudaStream_t st) {
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
   a.by_splits = FastDiv(a.splits);
   a.by_blocks = FastDiv(blocks);
-  launch_pdl(paged_rows_kernel<T, DP, W>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, a);
+  launch_pdl(paged_rows_kernel<T, DP, W, kEdge>, dim3((unsigned)grid), dim3(W * 32), C::kSmem, st, p, a);
   return launch_status("paged_rows");
 }
 
 template <typename T, int DP>
 static int launch_rows_dp(const Attn& p, RowsArgs a, cudaStream_t st) {
-  return a.two_warps ? launch_rows_w<T, DP, 2>(p, a, st) : launch_rows_w<T, DP, 4>(p, a, st);
+  if (a.phase != kPrefix && p.T > 1)
+    return a.two_warps ? launch_rows_w<T, DP, 2, true>(p, a, st) : launch_rows_w<T, DP, 4, true>(p, a, st);
+  return a.two_warps ? launch_rows_w<T, DP, 2, false>(p, a, st) : launch_rows_w<T, DP, 4, false>(p, a, st);
 }
 
 template <typename T>

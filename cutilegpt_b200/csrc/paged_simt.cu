@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Attn 
       l[i] = l[i] * a + warp_sum(e);
 #pragma unroll
       for (int k = 0; k < NC; ++k) acc[i][k] *= a;
-      for (int key = 0; key < kSimtKeys; ++key) {
+      for (int key = 0; key < min(kSimtKeys, seen[i] - j); ++key) {   // a value that the row does not see has no part in it
         const float w = __shfl_sync(0xffffffffu, e, key);
 #pragma unroll
         for (int k = 0; k < NC; ++k)

@@ -80,10 +80,11 @@ struct TcArgs {
   FastDiv by_splits, by_blocks, by_tile;
 };
 
-template <int D>
+// kEdge: several tokens a sequence and own keys, so that rows of a tile see different keys.
+template <int D, bool kEdge>
 __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_constant__ CUtensorMap tk,
-                                                                 const __grid_constant__ CUtensorMap tv, const Attn p,
-                                                                 const TcArgs a) {
+                                                                 const __grid_constant__ CUtensorMap tv,
+                                                                 const __grid_constant__ Attn p, const TcArgs a) {
   using C = Tc<D>;
   constexpr int ST = C::kStages;
   extern __shared__ uint8_t tc_smem_dyn[];
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
   uint64_t* pipe_bars = bars + 4 * ST;      // per pipeline: q_full, s_full, s_free, p_full (two halves), o_full
   uint64_t* turns = pipe_bars + 12;         // [pipeline][warp of the warpgroup]: its exponentials may begin
   uint32_t* tmem_slot = (uint32_t*)(turns + 8);
+  volatile uint32_t* again = tmem_slot + 1;            // the rows are computed again by slow_row
   float2* ml_smem = (float2*)((uint8_t*)bars + 512);   // [pipeline][row]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -135,6 +137,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       mbar_init(smem_addr(&b[5]), 1);
     }
     for (int i = 0; i < 8; ++i) mbar_init(smem_addr(&turns[i]), 1);
+    *again = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
@@ -186,10 +189,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       id = next;
       slot = next_slot;
       boxes = next_boxes;
+      if constexpr (kEdge) {
+        // values that some row of the block does not see: see slow_row. This warp has the time, and the slot
+        // is not filled again before it goes on.
+        const int t = t0 + i, at = (t - nt_pre) * a.tile, valid = min(a.tile, n_own - at);
+        const int edge = max(0, keys.n_own - p.T + p.by_share.div(r0) + 1);   // keys below: seen by all
+        if (is_v && t >= nt_pre && at + valid > edge) {
+          if (!mbar_wait(smem_addr(&full[st]), (uint32_t)((i / ST) & 1))) ok = false;
+          bool odd = false;
+#pragma unroll 4
+          for (int k = lane; k < valid * 8 * C::kPanels; k += 32) {
+            const int panel = k >= valid * 8;
+            odd |= non_finite<__nv_bfloat16>(
+                *reinterpret_cast<const uint4*>(ring + st * C::kTile + panel * kPanel + (k - panel * valid * 8) * 16));
+          }
+          if (odd) *again = 1;
+        }
+      }
     }
     // given up: the copies in flight land before the CTA's shared memory goes
     if (!ok)
       for (int j = max(0, i - ST); j < i; ++j) mbar_wait(smem_addr(&full[j % ST]), (uint32_t)((j / ST) & 1));
+    if (kEdge && is_v) {
+      __syncwarp();
+      asm volatile("bar.sync 2, 288;" ::: "memory");   // with the softmax warps: `again` is said
+    }
   } else if (warp >= 8) {
     // ------------------------------------------------ MMA issue, one lane per pipeline
     const int pipe = warp - 8;
@@ -421,6 +445,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       if (ok && !mbar_wait(smem_addr(&pb[5]), C::kAlias ? 0u : (uint32_t)((g - 1) & 1))) ok = false;
       tc_fence_after();
     }
+    bool done = false;
+    if constexpr (kEdge) {
+      asm volatile("bar.sync 2, 288;" ::: "memory");
+      done = *again != 0;
+      if (done) {   // an infinity or NaN at the causal edge: the block's rows once more, a warp for each
+        if (a.early) pdl_wait();
+        const int te = t0 + n_tiles;
+        const int j0 = t0 < nt_pre ? t0 * a.tile : keys.n_pre + (t0 - nt_pre) * a.tile;
+        const int j1 = te <= nt_pre ? min(keys.n_pre, te * a.tile) : keys.n_pre + min(n_own, (te - nt_pre) * a.tile);
+        for (int rr = r0 + warp; rr < min(rows, r0 + (a.two ? 256 : 128)); rr += 8) {
+          const Row to(p, b0, kh, rr);
+          const int end = keys.n_own - p.T + to.t;
+          float rm, rls, acc[4];
+          slow_row<__nv_bfloat16>(p, keys, kh, (const __nv_bfloat16*)p.q + to.b * p.q_b + to.h * p.q_h + to.t * p.q_t, j0,
+                                  end < 0 ? j0 : min(j1, keys.n_pre + end + 1), lane, rm, rls, acc);
+          const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to.b, to.t, to.h);
+          if (!a.direct && lane == 0) p.ml[at] = make_float2(rm, rls);
+          for (int c = 0; c < D / 32; ++c) {
+            if (a.direct)
+              ((__nv_bfloat16*)p.out)[to.b * p.o_b + to.h * p.o_h + to.t * p.o_t + lane + 32 * c] =
+                  __float2bfloat16_rn(rls == 0.f ? 0.f : acc[c] / rls);
+            else if (rls != 0.f)
+              p.acc[at * D + lane + 32 * c] = acc[c];
+          }
+        }
+      }
+    }
     // The row's result: out, or its slot of partial results. Two pipelines on the same rows see each
     // other's (m, l) through shared memory and O in TMEM (same lanes), and write half the columns each.
     float scale0 = 1.f, scale1 = 0.f;   // of this pipeline's O, of the other's
@@ -440,7 +491,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     if (a.early) pdl_wait();
     const Row to_row(p, b0, kh, live ? r : r0);
     const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to_row.b, to_row.t, to_row.h);
-    const bool mine = live && (a.two || shared_rows || pipe == 0), none = l == 0.f;
+    const bool mine = live && !done && (a.two || shared_rows || pipe == 0), none = l == 0.f;
     if (mine && !a.direct && (a.two || pipe == 0)) p.ml[at] = make_float2(m, l);
     if (a.direct) {
       const float inv = none ? 0.f : 1.f / l;
@@ -524,7 +575,7 @@ static int page_map(CUtensorMap* map, const void* pages, const Attn& p, int box)
   return GPT_OK;
 }
 
-template <int D>
+template <int D, bool kEdge>
 static int launch_tc_d(const Attn& p, TcArgs a, cudaStream_t st) {
   static bool done[64] = {false};
   static std::mutex mu;
@@ -533,7 +584,7 @@ static int launch_tc_d(const Attn& p, TcArgs a, cudaStream_t st) {
   {
     std::lock_guard<std::mutex> g(mu);
     if (dev >= 0 && dev < 64 && !done[dev]) {
-      cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<D>::kSmem);
+      cudaError_t e = cudaFuncSetAttribute(paged_tc_kernel<D, kEdge>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tc<D>::kSmem);
       if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
       done[dev] = true;
     }
@@ -552,12 +603,14 @@ static int launch_tc_d(const Attn& p, TcArgs a, cudaStream_t st) {
   a.by_splits = FastDiv(a.splits);
   a.by_blocks = FastDiv(blocks);
   a.by_tile = FastDiv(a.tile);
-  launch_pdl(paged_tc_kernel<D>, dim3((unsigned)grid), dim3(kTcThreads), Tc<D>::kSmem, st, mk, mv, p, a);
+  launch_pdl(paged_tc_kernel<D, kEdge>, dim3((unsigned)grid), dim3(kTcThreads), Tc<D>::kSmem, st, mk, mv, p, a);
   return launch_status("paged_tc");
 }
 
 static int launch_tc(const Attn& p, const TcArgs& a, cudaStream_t st) {
-  return p.D == 64 ? launch_tc_d<64>(p, a, st) : launch_tc_d<128>(p, a, st);
+  if (a.phase != kPrefix && p.T > 1)
+    return p.D == 64 ? launch_tc_d<64, true>(p, a, st) : launch_tc_d<128, true>(p, a, st);
+  return p.D == 64 ? launch_tc_d<64, false>(p, a, st) : launch_tc_d<128, false>(p, a, st);
 }
 
 }  // namespace paged

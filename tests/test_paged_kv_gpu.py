@@ -477,3 +477,24 @@ def test_append_many_tokens(dtype, interleaved, rot):
             assert ((have.double() - y).abs() <= (4 * 2.0 ** -24 * m + u * y.abs()) * (m > 0)).all()
         else:
             assert torch.equal(have, src)
+
+
+@pytest.mark.parametrize("case", [(BF, 3, 1, 4, 8, 2, 64, 16, [100], [4, 40, 77]), (F32, 3, 1, 4, 8, 2, 64, 16, [100], [4, 40, 77]),
+                                  (BF, 3, 1, 33, 4, 2, 64, 64, [190], [33, 40, 64]), (BF, 2, 1, 150, 4, 1, 128, 64, [260], [150, 400]),
+                                  (BF, 2, 0, 9, 2, 2, 128, 16, [], [9, 300]), (BF, 2, 1, 3, 2, 1, 7, 16, [20], [3, 30])],
+                         ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_attention_non_finite_values_of_later_tokens(case):
+    """Keys and values of a token that hold infinities and NaN reach its own row and later ones, no earlier one."""
+    kv, q = make(*case)
+    dtype, B, G, T, page = case[0], case[1], case[2], case[3], case[7]
+    seq, at = case[9], T // 2
+    clean, tol = reference(q, kv, q.shape[-1] ** -0.5)
+    for n, (pages, junk) in enumerate(((kv.v_pages, [float("inf"), float("nan")]), (kv.k_pages, [float("nan"), float("-inf")]))):
+        for b in range(B):
+            for t, x in zip((at, T - 1), junk):
+                i = seq[b] - T + t
+                pages[int(kv.page_table[b, i // page]), :, i % page] = x
+        got = cg.cutile_shared_prefix_attention(q, kv).double().cpu()
+        assert ((got[:, :, :at] - clean[:, :, :at]).abs() <= tol[:, :, :at]).all(), n
+        assert not got[:, :, T - 1].isfinite().all(), n
+    assert L.device_error() == 0
