@@ -293,7 +293,9 @@ GPT_API int gpt_sample(const void* logits, int64_t ld, int64_t B, int64_t V,
  * follows them. Table entries behind a length are not read, cache slots
  * behind it may hold anything. A page id outside [0, n_pages), a negative
  * length or one past the table's capacity is reported by gpt_device_error();
- * such a page reads as zeros and is not written, such a length is clamped. */
+ * such a page reads as zeros and is not written, such a length is clamped
+ * where it is read, and where tokens are written keeps their positions: those
+ * past the table are not written. */
 typedef struct gpt_paged_kv {
   void* k_pages;
   void* v_pages;
@@ -319,8 +321,8 @@ typedef struct gpt_paged_kv {
 /* T new tokens of each sequence into the cache, their rotation on the way.
  * Element (b, h, t, d) of q / q_out (H heads), k and v (kv_heads heads) is at
  * b*s[0] + h*s[1] + t*s[2] + d. Token t of sequence b has own position
- * i = seq_lens[b] - T + t; tokens with i < 0 are padding and are skipped
- * (their q_out rows are zeros). With rot > 0 the first rot values of every
+ * i = seq_lens[b] - T + t; tokens with i < 0 are padding and are skipped, as
+ * are those past the table (their q_out rows are zeros). With rot > 0 the first rot values of every
  * query and key head are turned by position n = (prefix length) + i:
  * pair j, (x[j], x[j + rot/2]) or with interleaved != 0 (x[2j], x[2j+1]),
  * becomes (x0*c - x1*s, x0*s + x1*c), c = cos_sin[n][j], s =
