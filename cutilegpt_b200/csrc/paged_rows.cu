@@ -489,15 +489,16 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
 #pragma unroll
     for (int u = 0; u < W; ++u) top = fmaxf(top, sm_ml[u * kRowTile + rl].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float2 ml, float4 x) {            // a part without keys has l = 0 and anything in x
-      const float w = ml.y == 0.f ? 0.f : exp2f(ml.x - top);
-      if (w != 0.f) {
-        sum = fmaf(ml.y, w, sum);
-        acc.x = fmaf(x.x, w, acc.x);
-        acc.y = fmaf(x.y, w, acc.y);
-        acc.z = fmaf(x.z, w, acc.z);
-        acc.w = fmaf(x.w, w, acc.w);
-      }
+    // A part without keys has l = 0 and anything in x. One whose scores are all NaN has m = -inf, as a maximum
+    // passes NaN over, but a NaN l: at the weight 0 it still joins.
+    auto add = [&](float2 ml, float4 x) {
+      if (ml.y == 0.f) return;
+      const float w = exp2f(ml.x - top);
+      sum = fmaf(ml.y, w, sum);
+      acc.x = fmaf(x.x, w, acc.x);
+      acc.y = fmaf(x.y, w, acc.y);
+      acc.z = fmaf(x.z, w, acc.z);
+      acc.w = fmaf(x.w, w, acc.w);
     };
 #pragma unroll
     for (int s = 0; s < 8; ++s)

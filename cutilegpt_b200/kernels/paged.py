@@ -139,10 +139,10 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
     q (batch, n_head, tokens, head_dim), k and v (batch, n_kv_head, tokens, head_dim), any strides with a
     contiguous head_dim (the parts of a fused projection are read in place). Token t of sequence b goes
     to own position seq_lens[b] - tokens + t; a negative one is padding and is skipped, one past the
-    table is skipped and reported by the device error word. cos_sin float32 [n_pos, rot]: cosines, then sines, of the rot / 2 angles of each position; the first rot values of
-    every query and key head are turned, in pairs (j, j + rot / 2) or, interleaved, (2j, 2j + 1), by the
-    position counted from the start of the prefix. q_out may be q itself; without cos_sin q is returned
-    as it is and may be None.
+    table is skipped and reported by the device error word. cos_sin float32 [n_pos, rot]: cosines, then
+    sines, of the rot / 2 angles of each position; the first rot values of every query and key head are
+    turned, in pairs (j, j + rot / 2) or, interleaved, (2j, 2j + 1), by the position counted from the start
+    of the prefix. q_out may be q itself; without cos_sin q is returned as it is and may be None.
     """
     k = _rows(k, "k", kv, kv.n_kv_head, None)
     tokens = k.shape[2]

@@ -1,12 +1,119 @@
-"""The paged key/value cache at the edges of its contract."""
+"""The paged key/value cache at the edges of its contract: infinities, NaN and huge values against the definition,
+lengths past a table, calls from several threads, outputs given by the caller.
+
+The tolerance of a finite result is that of test_paged_kv_gpu.py, with the keys of weight 0 (a score of -inf) left out
+of its largest score: A (2 u + off) in bf16, A (u + off) in fp32, A = sum_j p_j |v_j| and off = 2 (head_dim + 2) 2^-24 S
++ (n + 32) 2^-24. NaN and infinities have to be where the definition has them.
+"""
 import pytest
 import torch
 
 import cutilegpt_b200 as cg
 from cutilegpt_b200 import _lib as L
-from test_paged_kv_gpu import BF, F32, make
+from test_paged_kv_gpu import BF, F32, U, make
 
 pytestmark = pytest.mark.gpu
+NAN, INF = float("nan"), float("inf")
+
+
+def definition(q, kv, scale):
+    """fp64 outputs and tolerances, row by row: only what a row sees is looked at."""
+    B, H, T, D = q.shape
+    page = kv.k_pages.shape[2]
+    kp, vp, qc = kv.k_pages.double().cpu(), kv.v_pages.double().cpu(), q.double().cpu()
+    table, seq = kv.page_table.cpu().long(), kv.seq_lens.tolist()
+    G = kv.prefix_table.shape[0] if kv.prefix_table is not None else 0
+    out, tol = torch.zeros(B, H, T, D, dtype=torch.float64), torch.zeros(B, H, T, D, dtype=torch.float64)
+    for b in range(B):
+        i = torch.arange(seq[b])
+        pages, slots = table[b][i // page], i % page
+        if G:
+            g = b // (B // G)
+            i = torch.arange(int(kv.prefix_lens[g]))
+            pages = torch.cat([kv.prefix_table[g].cpu().long()[i // page], pages])
+            slots = torch.cat([i % page, slots])
+        for t in range(T):
+            if seq[b] - T + t < 0:
+                continue
+            n = len(pages) - T + t + 1
+            k, v = (x[pages[:n], :, slots[:n]].repeat_interleave(H // kv.n_kv_head, dim=1) for x in (kp, vp))
+            terms = qc[b, :, t] * k * scale                                  # [n, H, D]
+            s = terms.sum(-1)
+            S = torch.where(s.isfinite(), terms.abs().sum(-1), 0.0).amax(0)   # [H]
+            p = torch.softmax(s, 0)[..., None]
+            out[b, :, t] = (p * v).sum(0)
+            off = 2 * (D + 2) * 2.0 ** -24 * S + (n + 32) * 2.0 ** -24
+            tol[b, :, t] = (p * v.abs()).sum(0) * ((2 if q.dtype == BF else 1) * U[q.dtype] + off)[:, None]
+    return out, tol
+
+
+def check(q, kv, scale=None):
+    got = cg.cutile_shared_prefix_attention(q, kv, scale).double().cpu()
+    ref, tol = definition(q, kv, q.shape[-1] ** -0.5 if scale is None else scale)
+    assert torch.equal(got.isnan(), ref.isnan())
+    assert torch.equal(got.isinf(), ref.isinf()) and torch.equal(got[ref.isinf()], ref[ref.isinf()])
+    fin = ref.isfinite()
+    off = (got - ref).abs()[fin] / tol[fin].clamp_min(1e-300)
+    assert off.numel() == 0 or off.max() <= 1, f"off by {off.max().item()} of the tolerance"
+    assert L.device_error() == 0
+    return ref
+
+
+def spot(kv, b, i):
+    """Page and slot of own position i of sequence b."""
+    page = kv.k_pages.shape[2]
+    return int(kv.page_table[b, i // page]), i % page
+
+
+def prefix_spot(kv, g, i):
+    page = kv.k_pages.shape[2]
+    return int(kv.prefix_table[g, i // page]), i % page
+
+
+# ------------------------------------------------------------------ NaN in keys
+FEW_ROWS = [
+    # dtype, B, G, T, H, K, D, page, prefix, seq: served by the few-row kernel
+    (BF, 2, 0, 1, 4, 2, 64, 16, [], [17, 40]),
+    (BF, 2, 0, 1, 4, 2, 128, 16, [], [17, 65]),
+    (F32, 2, 0, 1, 4, 2, 64, 16, [], [17, 40]),
+    (BF, 2, 1, 1, 8, 4, 32, 16, [40], [17, 3]),
+    (BF, 3, 1, 1, 4, 4, 64, 16, [700], [5, 33, 17]),        # the prefix in slots of its own
+    (F32, 3, 1, 1, 2, 2, 128, 16, [700], [5, 33, 9]),
+    (BF, 1, 0, 3, 4, 4, 64, 16, [], [35]),
+]
+
+
+def nan_keys_one_by_one(case):
+    """NaN in the key of one position at a time, then in the keys of one page."""
+    kv, q = make(*case)
+    seq, prefix, page = case[9], case[8], case[7]
+    clean = kv.k_pages.clone()
+    for b, n in enumerate(seq):
+        for i in sorted({0, n // 2, n - 1}):
+            pid, slot = spot(kv, b, i)
+            kv.k_pages[pid, :, slot] = NAN
+            assert check(q, kv)[b].isnan().any()
+            kv.k_pages.copy_(clean)
+    for g, n in enumerate(prefix):
+        for i in sorted({0, n // 2, n - 1}):
+            pid, slot = prefix_spot(kv, g, i)
+            kv.k_pages[pid, :, slot] = NAN
+            assert check(q, kv).isnan().any()
+            kv.k_pages[pid] = NAN                             # a whole page
+            assert check(q, kv).isnan().any()
+            kv.k_pages.copy_(clean)
+
+
+@pytest.mark.parametrize("case", FEW_ROWS, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_nan_keys_few_rows(case):
+    """A key that is alone among what a warp, or a share of the keys, has met for a row."""
+    nan_keys_one_by_one(case)
+
+
+@pytest.mark.parametrize("case", [(BF, 3, 1, 1, 32, 1, 64, 16, [700], [5, 33, 17]), (BF, 1, 1, 40, 2, 1, 128, 64, [260], [140])],
+                         ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_nan_keys_many_rows(case):
+    nan_keys_one_by_one(case)
 
 
 # ------------------------------------------------------------------ append past a table
