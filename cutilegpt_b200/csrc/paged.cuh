@@ -154,7 +154,8 @@ __device__ __noinline__ void slow_row(const Attn& p, const Keys keys, int kh, co
     for (int c = 0; c < 4; ++c)
       if (off >= 0 && lane + 32 * c < p.D) s = fmaf(x[c], Tr<T>::to_f(((const T*)p.k)[off + lane + 32 * c]), s);
     s = warp_sum(s) * p.scale_log2;
-    const float to = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - to), e = to == -INFINITY ? 0.f : exp2f(s - to);
+    // a NaN score leaves m where it is, -inf at first: its exponential is NaN all the same
+    const float to = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - to), e = s == -INFINITY ? 0.f : exp2f(s - to);
     m = to;
     l = l * a + e;
     for (int c = 0; c < 4; ++c)

@@ -116,6 +116,22 @@ def test_nan_keys_many_rows(case):
     nan_keys_one_by_one(case)
 
 
+# ------------------------------------------------------------------ rows that are computed again
+@pytest.mark.parametrize("case", [(BF, 2, 0, 4, 4, 4, 64, 16, [], [20, 50]), (F32, 2, 0, 4, 4, 4, 64, 16, [], [20, 50]),
+                                  (BF, 1, 0, 40, 4, 1, 128, 64, [], [140])],
+                         ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_nan_keys_beside_infinite_values(case):
+    """An infinite value of the last token, and NaN in the first keys: every row sees these."""
+    kv, q = make(*case)
+    for b, n in enumerate(case[9]):
+        for i in (0, 1):
+            pid, slot = spot(kv, b, i)
+            kv.k_pages[pid, :, slot] = NAN
+        pid, slot = spot(kv, b, n - 1)
+        kv.v_pages[pid, :, slot] = INF
+    assert check(q, kv).isnan().all()
+
+
 # ------------------------------------------------------------------ append past a table
 @pytest.mark.parametrize("dtype,D,rot", [(BF, 64, 0), (BF, 64, 64), (F32, 64, 32), (BF, 7, 4), (F32, 7, 0)])
 @pytest.mark.parametrize("T,past", [(1, 1), (5, 2), (5, 5), (5, 100), (3, 2 ** 31 - 1 - 48)])
