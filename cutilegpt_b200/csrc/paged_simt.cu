@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kSimtWarps * 32) paged_simt_kernel(const Attn 
       if (j + lane >= min(seen[i], j1)) s = -INFINITY;
       const float mn = fmaxf(m[i], warp_max(s));
       const float a = m[i] == -INFINITY ? 0.f : exp2f(m[i] - mn);
-      const float e = mn == -INFINITY ? 0.f : exp2f(s - mn);
+      const float e = s == -INFINITY ? 0.f : exp2f(s - mn);   // NaN for a NaN score, which leaves the maximum alone
       m[i] = mn;
       l[i] = l[i] * a + warp_sum(e);
 #pragma unroll

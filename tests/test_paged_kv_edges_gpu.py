@@ -132,6 +132,31 @@ def test_nan_keys_beside_infinite_values(case):
     assert check(q, kv).isnan().all()
 
 
+# ------------------------------------------------------------------ the kernel for all other sizes
+SIMT = [
+    (BF, 2, 0, 1, 3, 1, 7, 16, [], [40, 33]),
+    (F32, 2, 0, 1, 3, 1, 7, 16, [], [70, 20]),
+    (F32, 1, 0, 2, 2, 1, 7, 16, [], [3000]),                 # dozens of shares
+    (BF, 2, 1, 1, 4, 2, 256, 16, [40], [3, 20]),
+]
+
+
+@pytest.mark.parametrize("case", SIMT, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_nan_keys_any_size(case):
+    """NaN in the first keys, as many as a step takes, and in all of a query."""
+    kv, q = make(*case)
+    clean = kv.k_pages.clone()
+    for b, n in enumerate(case[9]):
+        for i in range(min(32, n)):
+            pid, slot = spot(kv, b, i)
+            kv.k_pages[pid, :, slot] = NAN
+    assert check(q, kv).isnan().all()
+    kv.k_pages.copy_(clean)
+    q = q.clone()
+    q[0, 0] = NAN
+    assert check(q, kv)[0, 0].isnan().all()
+
+
 # ------------------------------------------------------------------ append past a table
 @pytest.mark.parametrize("dtype,D,rot", [(BF, 64, 0), (BF, 64, 64), (F32, 64, 32), (BF, 7, 4), (F32, 7, 0)])
 @pytest.mark.parametrize("T,past", [(1, 1), (5, 2), (5, 5), (5, 100), (3, 2 ** 31 - 1 - 48)])
