@@ -509,9 +509,10 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     for (int u = 0; u < W; ++u)
       add(sm_ml[u * kRowTile + rl], *reinterpret_cast<const float4*>(sm_o + (u * kRowTile + rl) * DP + d));
     if (a.direct) {
-      const float inv = sum == 0.f || keys.n_own - p.T + at.t < 0 ? 0.f : 1.f / sum;   // 0: padding
+      const bool padding = keys.n_own - p.T + at.t < 0;
+      const float inv = 1.f / sum;   // sum = 0: every score is -inf, the row is 0 / 0
       store4((T*)p.out + at.b * p.o_b + at.h * p.o_h + at.t * p.o_t + d,
-             inv == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+             padding ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     } else {
       const int64_t to = (int64_t)(a.slot0 + split) * all_rows + row;
       if (d == 0) p.ml[to] = make_float2(top, sum);

@@ -208,10 +208,11 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Attn p, 
   }
   if (!mine || group != 0) return;
   const int h = (int)(row % p.H), t = (int)(row / p.H % p.T), b = (int)(row / p.H / p.T);
-  const float inv = l == 0.f || last_key(p, b, t) < 0 ? 0.f : 1.f / l;   // 0: padding
+  const bool padding = last_key(p, b, t) < 0;
+  const float inv = 1.f / l;   // l = 0: every score is -inf, the row is 0 / 0
   T* out = (T*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d;
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = Tr<T>::from_f(inv == 0.f ? 0.f : acc.c[i] * inv);
+  for (int i = 0; i < V; ++i) out[i] = Tr<T>::from_f(padding ? 0.f : acc.c[i] * inv);
 }
 
 template <typename T, int RB>

@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
           for (int c = 0; c < D / 32; ++c) {
             if (a.direct)
               ((__nv_bfloat16*)p.out)[to.b * p.o_b + to.h * p.o_h + to.t * p.o_t + lane + 32 * c] =
-                  __float2bfloat16_rn(rls == 0.f ? 0.f : acc[c] / rls);
+                  __float2bfloat16_rn(end < 0 ? 0.f : acc[c] / rls);
             else if (rls != 0.f)
               p.acc[at * D + lane + 32 * c] = acc[c];
           }
@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
     const Row to_row(p, b0, kh, live ? r : r0);
     const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to_row.b, to_row.t, to_row.h);
     const bool mine = live && !done && (a.two || shared_rows || pipe == 0), none = l == 0.f;
+    const uint32_t no_keys = last < 0 ? 0u : 0x7fc07fc0u;   // zeros for padding, else every score is -inf: 0 / 0
     if (mine && !a.direct && (a.two || pipe == 0)) p.ml[at] = make_float2(m, l);
     if (a.direct) {
       const float inv = none ? 0.f : 1.f / l;
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
           uint32_t w[4];
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            w[u] = none ? 0u : tc::pack2_bf16(__uint_as_float(o[8 * k + 2 * u]), __uint_as_float(o[8 * k + 2 * u + 1]));
+            w[u] = none ? no_keys : tc::pack2_bf16(__uint_as_float(o[8 * k + 2 * u]), __uint_as_float(o[8 * k + 2 * u + 1]));
           dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
         }
       } else if (!none) {

@@ -157,6 +157,28 @@ def test_nan_keys_any_size(case):
     assert check(q, kv)[0, 0].isnan().all()
 
 
+# ------------------------------------------------------------------ scores of -inf
+ALL_KERNELS = FEW_ROWS + SIMT + [
+    (BF, 40, 1, 1, 2, 1, 64, 16, [517], [1 + i % 5 for i in range(40)]),     # 128-row tiles, the prefix in slots
+    (BF, 1, 0, 150, 2, 1, 128, 64, [], [150]),
+    (BF, 2, 1, 33, 2, 1, 64, 64, [190], [40, 33]),
+    (BF, 1, 0, 300, 1, 1, 64, 64, [], [300]),
+]
+
+
+@pytest.mark.parametrize("case", ALL_KERNELS, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_rows_without_a_finite_score(case):
+    """Every score of a row is -inf: 0 / 0, whichever kernel serves the call; padding stays zeros."""
+    kv, q = make(*case, garbage=False)
+    q = q.clone()
+    q[..., 0] = q[..., 0].abs() + 0.5
+    kv.k_pages[..., 0] = -INF
+    assert check(q, kv).isnan().all()
+    kv.seq_lens[0] = 0
+    ref = check(q, kv)
+    assert (ref[0] == 0).all() and ref[1:].isnan().all()
+
+
 # ------------------------------------------------------------------ append past a table
 @pytest.mark.parametrize("dtype,D,rot", [(BF, 64, 0), (BF, 64, 64), (F32, 64, 32), (BF, 7, 4), (F32, 7, 0)])
 @pytest.mark.parametrize("T,past", [(1, 1), (5, 2), (5, 5), (5, 100), (3, 2 ** 31 - 1 - 48)])
