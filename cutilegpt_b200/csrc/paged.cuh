@@ -2,6 +2,8 @@
 // partial results are, shared by paged_append.cu, paged_simt.cu and paged.cu.
 #pragma once
 
+#include <float.h>
+
 #include "common.cuh"
 
 namespace gpt {
@@ -120,6 +122,14 @@ struct Keys {
     return id < 0 ? -1 : id * p.page_stride + kh * p.head_stride + (int64_t)(i - at * p.page) * p.slot_stride;
   }
 };
+
+// A column's mean of values, acc times inv = 1 / l. The largest fp32 numbers come out of their split parts rounded
+// up by 2^-24 (paged_rows.cu), past the range; a mean is never past it.
+template <typename T>
+__device__ __forceinline__ float mean(float acc, float inv) {
+  const float x = acc * inv;
+  return sizeof(T) == 4 && isinf(x) && !isinf(acc) ? copysignf(FLT_MAX, x) : x;
+}
 
 // ---- infinities and NaN in values that not every row of a tile sees -----------
 // The tensor-core kernels give such a value the probability 0 for the rows that do not see it, and multiply:

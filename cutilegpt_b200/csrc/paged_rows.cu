@@ -109,16 +109,23 @@ __device__ __forceinline__ uint32_t to_tf32(float x) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
   return r;
 }
+// hi is never rounded to infinity: of a number near the largest it is the largest TF32, of an infinity too, and lo
+// is the rest, an infinity then. Products with both parts thus have the infinity once; NaN is NaN in both.
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  hi = to_tf32(x);
+  asm("cvt.rna.satfinite.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
   lo = to_tf32(x - __uint_as_float(hi));
 }
-// c += a b in three TF32 products, the small ones first.
+// c += a b in three TF32 products, the small ones first. kLarge: a may exceed 1 so far that its low part by an
+// infinity's high one overflows against the infinity's sign: that product is left out.
+template <bool kLarge>
 __device__ __forceinline__ void mma_split(float (&c)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4], float b0, float b1) {
   uint32_t h0, l0, h1, l1;
   split_tf32(b0, h0, l0);
   split_tf32(b1, h1, l1);
-  mma1688(c, al, h0, h1);
+  if (kLarge)
+    mma1688(c, al, isinf(b0) ? 0u : h0, isinf(b1) ? 0u : h1);
+  else
+    mma1688(c, al, h0, h1);
   mma1688(c, ah, l0, l1);
   mma1688(c, ah, h0, h1);
 }
@@ -300,8 +307,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
         for (int i = 0; i < KS / 8; ++i) {
           float kv[4], part[4] = {0.f, 0.f, 0.f, 0.f};
           lds128(sk + swz<T, DP>(i * 8 + lane / 4, k * 4 + quad), kv);
-          mma_split(part, ah[0], al[0], kv[0], kv[1]);
-          mma_split(part, ah[1], al[1], kv[2], kv[3]);
+          mma_split<true>(part, ah[0], al[0], kv[0], kv[1]);
+          mma_split<true>(part, ah[1], al[1], kv[2], kv[3]);
 #pragma unroll
           for (int u = 0; u < 4; ++u) sc[i][u] += part[u];
         }
@@ -337,7 +344,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * p.scale_log2;
+      // fp32: P is at most 1/2, so that a value near the largest number stays in range while its parts are added
+      mx[h] = fmaf(fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)), p.scale_log2, kWide ? 1.f : 0.f);
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
       float by[2];
@@ -380,7 +388,7 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
           lds128(sv + swz<T, DP>(i * 8 + 2 * quad, d * 8 + lane / 4), v0);
           lds128(sv + swz<T, DP>(i * 8 + 2 * quad + 1, d * 8 + lane / 4), v1);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) mma_split(part[u], ah[i], al[i], v0[u], v1[u]);
+          for (int u = 0; u < 4; ++u) mma_split<false>(part[u], ah[i], al[i], v0[u], v1[u]);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -512,7 +520,8 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
       const bool padding = keys.n_own - p.T + at.t < 0;
       const float inv = 1.f / sum;   // sum = 0: every score is -inf, the row is 0 / 0
       store4((T*)p.out + at.b * p.o_b + at.h * p.o_h + at.t * p.o_t + d,
-             padding ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+             padding ? make_float4(0.f, 0.f, 0.f, 0.f)
+                     : make_float4(mean<T>(acc.x, inv), mean<T>(acc.y, inv), mean<T>(acc.z, inv), mean<T>(acc.w, inv)));
     } else {
       const int64_t to = (int64_t)(a.slot0 + split) * all_rows + row;
       if (d == 0) p.ml[to] = make_float2(top, sum);

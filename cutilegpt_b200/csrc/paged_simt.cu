@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const Attn p, 
   const float inv = 1.f / l;   // l = 0: every score is -inf, the row is 0 / 0
   T* out = (T*)p.out + b * p.o_b + h * p.o_h + t * p.o_t + d;
 #pragma unroll
-  for (int i = 0; i < V; ++i) out[i] = Tr<T>::from_f(padding ? 0.f : acc.c[i] * inv);
+  for (int i = 0; i < V; ++i) out[i] = Tr<T>::from_f(padding ? 0.f : mean<T>(acc.c[i], inv));
 }
 
 template <typename T, int RB>

@@ -179,6 +179,64 @@ def test_rows_without_a_finite_score(case):
     assert (ref[0] == 0).all() and ref[1:].isnan().all()
 
 
+# ------------------------------------------------------------------ infinite and huge operands in fp32
+FP32 = [
+    (F32, 2, 0, 1, 4, 2, 64, 16, [], [17, 40]),
+    (F32, 3, 1, 1, 2, 2, 128, 16, [700], [5, 33, 9]),
+    (F32, 3, 1, 4, 4, 2, 32, 16, [50], [4, 20, 77]),
+    (F32, 2, 0, 1, 3, 1, 7, 16, [], [17, 40]),               # the plain kernel
+]
+
+
+@pytest.mark.parametrize("case", FP32, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_fp32_infinite_keys_and_values(case):
+    kv, q = make(*case, garbage=False)
+    T, seq = case[3], case[9]
+    clean = kv.k_pages.clone(), kv.v_pages.clone()
+    q = q.clone()
+    # first elements that fill fp32, that have 11 bits, and that lie just below and above such a number
+    first = torch.tensor([0.7, 1.0, 1.5 - 2.0 ** -20, 1.5 + 2.0 ** -20, 4097.0 - 2.0 ** -9], device="cuda")
+    q[..., 0] = first[torch.arange(q[..., 0].numel(), device="cuda") % 5].view(q.shape[:3])
+    for b, n in enumerate(seq):
+        pid, slot = spot(kv, b, (n - T) // 2)
+        kv.k_pages[pid, :, slot, 0] = -INF                    # weight 0
+        kv.v_pages[pid, :, slot] = 1000.0
+    kv.k_pages[..., 0].clamp_(-INF, 1e-3)
+    assert check(q, kv, 0.01).isfinite().all()
+    for b, n in enumerate(seq):                               # seen by every row: +inf, -inf, and both
+        for i, x in ((0, INF), (1, -INF)):
+            pid, slot = spot(kv, b, max(0, min(i, n - T)))
+            kv.k_pages[pid, :, slot] = 0.0
+            kv.v_pages[pid, :, slot, 2 * i:2 * i + 3] = x
+    ref = check(q, kv, 0.01)
+    assert ref.isinf().any() and not ref.isnan().all()
+    kv.k_pages.copy_(clean[0])
+    kv.v_pages.copy_(clean[1])
+    big = 3.4028234e38
+    for b, n in enumerate(seq):                               # the largest number, of either sign, in one key's values
+        pid, slot = spot(kv, b, n - 1)
+        kv.v_pages[pid, :, slot, 0] = big
+        kv.v_pages[pid, :, slot, 1] = -big
+    assert check(q, kv, 0.01).isfinite().all()
+
+
+@pytest.mark.parametrize("n,D", [(1, 64), (1, 128), (33, 32), (700, 64)])
+def test_fp32_largest_numbers(n, D):
+    """One key has all the weight, and its values are the largest numbers."""
+    kv, q = make(F32, 1, 0, 1, 2, 2, D, 16, [], [n])
+    q = torch.zeros_like(q)
+    q[..., 0] = 1.0
+    top = torch.tensor([3.4028235e38, 3.4028233e38, 3.402e38, -3.4028235e38], device="cuda")
+    kv.k_pages[..., 0] = 0.0
+    for i in {0, n // 2, n - 1}:
+        pid, slot = spot(kv, 0, i)
+        kv.k_pages[pid, :, slot, 0] = 900.0
+        kv.v_pages[pid, :, slot] = top[torch.arange(D, device="cuda") % 4]
+        assert check(q, kv, 0.5).isfinite().all()
+        kv.k_pages[pid, :, slot, 0] = 0.0
+        kv.v_pages[pid, :, slot] = 1.0
+
+
 # ------------------------------------------------------------------ append past a table
 @pytest.mark.parametrize("dtype,D,rot", [(BF, 64, 0), (BF, 64, 64), (F32, 64, 32), (BF, 7, 4), (F32, 7, 0)])
 @pytest.mark.parametrize("T,past", [(1, 1), (5, 2), (5, 5), (5, 100), (3, 2 ** 31 - 1 - 48)])
