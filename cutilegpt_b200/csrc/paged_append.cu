@@ -87,15 +87,15 @@ __device__ __forceinline__ void append_one(const Append& p, int b, int id) {
   }
 
   const int pre = p.plens ? clamped_len(p.plens, b / p.per, p.pcap) : 0;
-  // A length past the table keeps its tokens' positions, and those without a slot go nowhere: clamped like a length
-  // that is only read, the new tokens would land on earlier ones.
-  const int len = p.seq_lens[b], i = max(len, 0) - p.T + t;
+  // A length past the table keeps its tokens' positions, and those without a slot are treated as padding: clamped like a
+  // length that is only read, the new tokens would land on earlier ones.
+  const int len = p.seq_lens[b], at = max(len, 0) - p.T + t, i = at < p.cap ? at : -1;
   if (len < 0 || len > p.cap) record_device_error(GPT_DEVERR_INDEX);
   T* dst;
   if (kind == 2) {
     dst = (T*)p.q_out + b * p.o_s[0] + h * p.o_s[1] + t * p.o_s[2];
   } else {
-    if (i < 0 || i >= p.cap) return;   // padding, no slot
+    if (i < 0) return;   // padding
     const int page = p.by_page.div(i), pid = page_id(p.table[b * p.ld_table + page], p.n_pages);
     if (pid < 0) return;
     dst = (T*)(kind == 0 ? p.k_pages : p.v_pages) + pid * p.page_stride + h * p.head_stride +
@@ -103,9 +103,8 @@ __device__ __forceinline__ void append_one(const Append& p, int b, int id) {
   }
   if (rot > 0) {
     const int64_t n = (int64_t)pre + i;
-    // a position without a table row gives a row of zeros, its unrotated part included, as does a query of a padding
-    // token or of one without a slot
-    const bool known = i >= 0 && i < p.cap && n < p.n_pos;
+    // a position without a table row gives a row of zeros, its unrotated part included, as does a padding query
+    const bool known = i >= 0 && n < p.n_pos;
     if (i >= 0 && !known) record_device_error(GPT_DEVERR_INDEX);
     const float* cs = p.cos_sin + n * rot;
     using F = Vec<float, V % 4 == 0 ? 4 : 1>;
