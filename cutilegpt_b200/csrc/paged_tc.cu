@@ -17,10 +17,10 @@
 //   O += P V      A = P from TMEM, B = V MN-major as its boxes arrive; only the 16-key steps
 //                 that hold keys are issued, and the last one's rows behind the keys are cleared
 //                 first: what the cache holds there must not meet P = 0
-// The exponentials do not wait for the tile's maximum: m is what earlier tiles left,
-// P = 2^(s - m) may exceed 1 (fp32 and bf16 have the range), a tile whose maximum lies 2^8 above m
-// makes the next tile move m (O and the sum are rescaled), one 2^64 above moves it at once and
-// starts over. The PV of a tile's first 64 keys runs under the exponentials of the others. With D = 64 P has
+// The exponentials do not wait for the tile's maximum: m is 16 above the largest score (in powers of two) that earlier
+// tiles left, a tile whose maximum lies 8 above that one makes the next tile move m (O and the sum are rescaled), one
+// 16 above moves it at once and starts over. P = 2^(s - m) is thus at most 1, and a value of any size stays in range;
+// weights below 2^-110 of the largest are 0. The PV of a tile's first 64 keys runs under the exponentials of the others. With D = 64 P has
 // TMEM columns of its own and the next S is computed under the softmax; with D = 128
 // P takes the place of S (256 columns a pipeline), and the next S follows the PV.
 // Keys and values have separate rings; every wait is bounded.
@@ -60,8 +60,8 @@ using tc::tmem_ld32;
 
 constexpr int kTcThreads = 12 * 32;      // 2 x 4 softmax warps, 2 MMA warps, K and V copy warps
 constexpr int kPanel = 128 * 128;        // 128 rows of 64 bf16, 128-byte swizzled
-constexpr float kTcRescale = 8.f;        // log2 of the P from which the next tile moves m
-constexpr float kTcFar = 64.f;           // log2 of the P from which the tile itself moves m and starts over
+constexpr float kTcRescale = 8.f;        // rise of the largest score, in powers of two, from which the next tile moves m
+constexpr float kTcFar = 16.f;           // and from which the tile itself moves m and starts over; m lies this far above
 
 template <int D>
 struct Tc {
@@ -358,9 +358,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
           rescale = g > 0;
         };
         if (g == 0)
-          m = row_max();
-        else if (top > m + kTcRescale)
-          move_to(top);
+          m = row_max() + kTcFar;
+        else if (top > m + (kTcRescale - kTcFar))
+          move_to(top + kTcFar);
         // The two warps of a scheduler take turns at the exponentials, pipeline 0 first: while one's fill
         // the special-function unit the other's products run. Left alone the pipelines fall into step
         // and neither overlaps the other.
@@ -385,8 +385,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
         };
         exps(0, true);
         const float mx = row_max();   // beside the exponentials
-        if (__any_sync(0xffffffffu, mx > m + kTcFar)) {
-          if (mx > m + kTcFar) move_to(mx);
+        if (__any_sync(0xffffffffu, mx > m)) {
+          if (mx > m) move_to(mx + kTcFar);
           load(64);
           exps(0, true);
         }

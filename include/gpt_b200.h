@@ -348,7 +348,9 @@ GPT_API int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H,
  * h / (H / kv_heads). Rows of padding tokens (seq_lens[b] - T + t < 0) are
  * zeros; a row whose every score is -inf is NaN. Infinities and NaN reach the
  * rows that see them and no others (where a value of a new token holds one,
- * the rows of its CTA are computed again, slowly). What the sequences of a group share is read once for all of them;
+ * the rows of its CTA are computed again, slowly). Weighted values are summed
+ * in fp32 before the division: values near the largest number may overflow
+ * where several keys share the weight. What the sequences of a group share is read once for all of them;
  * parts of the keys are computed apart and joined through `workspace`
  * (gpt_attention_shared_prefix_workspace_size bytes, 16-byte aligned; NULL
  * when that is 0). scale must be positive and finite. Strides as above. */

@@ -237,6 +237,38 @@ def test_fp32_largest_numbers(n, D):
         kv.v_pages[pid, :, slot] = 1.0
 
 
+# ------------------------------------------------------------------ the range of values
+RISING = [
+    # enough sequences, groups and key heads that a CTA sees several tiles
+    (BF, 40, 0, 17, 2, 2, 64, 64, [], [700 - i for i in range(40)]),
+    (BF, 40, 0, 17, 2, 2, 128, 64, [], [700 - i for i in range(40)]),
+    (BF, 40, 0, 17, 16, 2, 64, 64, [], [450 - i for i in range(40)]),        # 256 rows on the same tiles
+    (BF, 40, 0, 17, 16, 2, 128, 64, [], [450 - i for i in range(40)]),
+    (BF, 80, 40, 1, 18, 2, 64, 64, [600] * 40, [1 + i % 5 for i in range(80)]),
+    (BF, 4, 1, 1, 2, 2, 64, 16, [517], [1, 2, 40, 300]),                     # the few-row kernel
+]
+
+
+@pytest.mark.parametrize("exponent", [100, -100])
+@pytest.mark.parametrize("case", RISING, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_large_values_behind_rising_scores(case, exponent):
+    """Values of 2^100 whose scores rise by 12 to 27 (in powers of two) from tile to tile: the weights of the first
+    tiles are what the sums are in units of until the kernel notices. And small values, which must not get lost."""
+    kv, q = make(*case, garbage=False)
+    page = case[7]
+    q = torch.zeros_like(q)
+    q[..., 0] = 1.0
+    lists = [(kv.page_table[b], n) for b, n in enumerate(case[9])] + [(kv.prefix_table[g], n) for g, n in enumerate(case[8])]
+    for row, n in lists:
+        level = 0
+        for i, pid in zip(range(0, n, page), row.tolist()):
+            if i % 128 == 0 and i > 0:
+                level += 10 + (i // 128 * 17) % 20
+            kv.k_pages[pid, ..., 0] = level
+    kv.v_pages.mul_(2.0 ** exponent)
+    assert check(q, kv, 0.693).isfinite().all()
+
+
 # ------------------------------------------------------------------ append past a table
 @pytest.mark.parametrize("dtype,D,rot", [(BF, 64, 0), (BF, 64, 64), (F32, 64, 32), (BF, 7, 4), (F32, 7, 0)])
 @pytest.mark.parametrize("T,past", [(1, 1), (5, 2), (5, 5), (5, 100), (3, 2 ** 31 - 1 - 48)])
