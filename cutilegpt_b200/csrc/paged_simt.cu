@@ -221,11 +221,22 @@ static int launch_simt_rb(const Attn& p, int phase, int splits, int slot0, int d
   const int64_t blocks = (rows + RB - 1) / RB;
   const int64_t grid = blocks * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
   GPT_CHECK_SHAPE(grid < (1LL << 31), "gpt_attention_shared_prefix: too many rows for one call");
-  const size_t smem = (size_t)(2 * kSimtKeys * (p.D | 1) + RB * p.D) * sizeof(float);
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(paged_simt_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  constexpr auto bytes = [](int D) { return (2 * kSimtKeys * (D | 1) + RB * D) * (int)sizeof(float); };
+  // The limit belongs to the kernel on the device, not to the call: the largest head's, once, as a smaller one set by
+  // another thread would have this launch refused.
+  static bool done[64] = {false};
+  static std::mutex mu;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  {
+    std::lock_guard<std::mutex> g(mu);
+    if (dev >= 0 && dev < 64 && !done[dev]) {
+      cudaError_t e = cudaFuncSetAttribute(paged_simt_kernel<T, RB>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes(kSimtMaxD));
+      if (e != cudaSuccess) return fail(GPT_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+      done[dev] = true;
+    }
   }
+  const size_t smem = bytes(p.D);
   launch_pdl(paged_simt_kernel<T, RB>, dim3((unsigned)grid), dim3(kSimtWarps * 32), smem, st, p, phase, splits,
              (int)blocks, slot0, direct);
   return launch_status("paged_simt");

@@ -5,6 +5,8 @@ The tolerance of a finite result is that of test_paged_kv_gpu.py, with the keys 
 of its largest score: A (2 u + off) in bf16, A (u + off) in fp32, A = sum_j p_j |v_j| and off = 2 (head_dim + 2) 2^-24 S
 + (n + 32) 2^-24. NaN and infinities have to be where the definition has them.
 """
+import threading
+
 import pytest
 import torch
 
@@ -304,3 +306,33 @@ def test_append_past_the_table(dtype, D, rot, T, past):
     assert L.device_error() == 0
     assert torch.equal(after[0], kv.k_pages) and torch.equal(after[1], kv.v_pages)
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------ calls from several threads
+def test_attention_from_several_threads():
+    """Head sizes whose tiles need different amounts of shared memory, at the same time."""
+    calls, kept = [], []
+    for D in (256, 160, 200, 136) * 2:
+        kv, q = make(F32, 2, 1, 5, 4, 1, D, 16, [40], [5, 20])
+        want, out = cg.cutile_shared_prefix_attention(q, kv), torch.zeros(q.shape, device="cuda")
+        ws = torch.empty(max(16, kv.workspace_bytes(4, 5)), dtype=torch.uint8, device="cuda")
+        stream = torch.cuda.Stream()
+        calls.append((q.data_ptr(), L.strides3(*q.stride()[:3]), out.data_ptr(), L.strides3(*out.stride()[:3]), 5, 4, kv._ref,
+                      D ** -0.5, ws.data_ptr(), ws.numel(), L.GPT_F32, stream.cuda_stream))
+        kept.append((kv, q, want, out, ws, stream))
+    torch.cuda.synchronize()
+    statuses, attend = [], L.lib().gpt_attention_shared_prefix
+
+    def work(args):
+        statuses.extend({attend(*args) for _ in range(2000)})
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert set(statuses) == {L.GPT_OK}
+    for _, _, want, out, _, _ in kept:
+        assert torch.equal(out, want)
+    assert L.device_error() == 0
