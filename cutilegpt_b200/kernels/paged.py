@@ -128,6 +128,8 @@ def _rows(t, name: str, kv: PagedKV, heads: int | None, tokens: int | None) -> t
 
 
 def _out_rows(t, name: str, kv: PagedKV, heads: int, tokens: int) -> torch.Tensor:
+    if type(t) is not torch.Tensor:
+        t = as_cuda(t, name)
     if _rows(t, name, kv, heads, tokens) is not t:
         raise ValueError(f"{name}: head_dim must be contiguous")
     return t
@@ -161,7 +163,7 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _out_rows(q_out, "q_out", kv, q.shape[1], tokens)
+        q_out = _out_rows(q_out, "q_out", kv, q.shape[1], tokens)
     ops.paged_kv_append(q, k, v, q_out, kv, cos_sin, interleaved)
     return q_out
 
@@ -183,5 +185,5 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _out_rows(out, "out", kv, heads, tokens)
+        out = _out_rows(out, "out", kv, heads, tokens)
     return ops.shared_prefix_attention(q, kv, out, dim ** -0.5 if scale is None else scale, workspace)

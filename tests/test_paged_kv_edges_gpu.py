@@ -336,3 +336,30 @@ def test_attention_from_several_threads():
     for _, _, want, out, _, _ in kept:
         assert torch.equal(out, want)
     assert L.device_error() == 0
+
+
+# ------------------------------------------------------------------ outputs given by the caller
+class Producer:
+    """An array of another library: DLPack and nothing else."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __dlpack__(self, **kw):
+        return self.t.__dlpack__(**kw)
+
+    def __dlpack_device__(self):
+        return self.t.__dlpack_device__()
+
+
+def test_outputs_of_another_library():
+    kv, q = make(BF, 3, 1, 2, 4, 2, 64, 16, [40], [3, 17, 30])
+    want = cg.cutile_shared_prefix_attention(q, kv)
+    out = torch.empty(q.shape, dtype=BF, device="cuda")
+    got = cg.cutile_shared_prefix_attention(q, kv, out=Producer(out))
+    assert torch.equal(out, want) and torch.equal(got, want)
+    k = torch.randn(3, 2, 2, 64, device="cuda").to(BF)
+    table = torch.randn(100, 64, device="cuda")
+    want = cg.cutile_paged_kv_append(q, k, k, kv, table)
+    got = cg.cutile_paged_kv_append(q, k, k, kv, table, q_out=Producer(out))
+    assert torch.equal(out, want) and torch.equal(got, want)
