@@ -144,7 +144,8 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
     table is skipped and reported by the device error word. cos_sin float32 [n_pos, rot]: cosines, then
     sines, of the rot / 2 angles of each position; the first rot values of every query and key head are
     turned, in pairs (j, j + rot / 2) or, interleaved, (2j, 2j + 1), by the position counted from the start
-    of the prefix. q_out may be q itself; without cos_sin q is returned as it is and may be None.
+    of the prefix. q_out may be q itself (same strides), and overlaps q in no other way; without cos_sin
+    q is returned as it is and may be None.
     """
     k = _rows(k, "k", kv, kv.n_kv_head, None)
     tokens = k.shape[2]
@@ -164,6 +165,9 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         q_out = _out_rows(q_out, "q_out", kv, q.shape[1], tokens)
+        if (q_out.data_ptr() == q.data_ptr() and q.numel()
+                and any(n > 1 and a != b for n, a, b in zip(q.shape, q.stride(), q_out.stride()))):
+            raise ValueError(f"q_out: in q's memory it needs q's strides {q.stride()}, got {q_out.stride()}")
     ops.paged_kv_append(q, k, v, q_out, kv, cos_sin, interleaved)
     return q_out
 
@@ -175,7 +179,7 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
     h // (n_head // n_kv_head)); token t of sequence b sees the prefix and its own positions 0 ..
     seq_lens[b] - tokens + t, and gives zeros where that is negative (padding, idle sequences). The prefix
     is read once for all sequences of its group. scale is 1/√head_dim by default. A new contiguous tensor is
-    returned unless `out` (any strides, contiguous head_dim, not q's memory) is given; `workspace` (uint8,
+    returned unless `out` (any strides, contiguous head_dim, no overlap with q) is given; `workspace` (uint8,
     kv.workspace_bytes(n_head, tokens)) is allocated unless given.
     """
     q = _rows(q, "q", kv, None, None)
@@ -186,4 +190,6 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         out = _out_rows(out, "out", kv, heads, tokens)
+        if out.data_ptr() == q.data_ptr() and q.numel():
+            raise ValueError("out: must not be q's memory")
     return ops.shared_prefix_attention(q, kv, out, dim ** -0.5 if scale is None else scale, workspace)

@@ -363,3 +363,22 @@ def test_outputs_of_another_library():
     want = cg.cutile_paged_kv_append(q, k, k, kv, table)
     got = cg.cutile_paged_kv_append(q, k, k, kv, table, q_out=Producer(out))
     assert torch.equal(out, want) and torch.equal(got, want)
+
+
+def test_outputs_in_the_way_are_refused():
+    kv, q = make(BF, 3, 1, 2, 4, 2, 64, 16, [40], [3, 17, 30])
+    with pytest.raises(ValueError, match="memory"):
+        cg.cutile_shared_prefix_attention(q, kv, out=q)
+    square = torch.randn(3, 2, 2, 64, device="cuda").to(BF)
+    kv2 = cg.PagedKV(kv.k_pages, kv.v_pages, kv.page_table, kv.seq_lens)
+    table = torch.randn(100, 64, device="cuda")
+    with pytest.raises(ValueError, match="strides"):
+        cg.cutile_paged_kv_append(square, square.clone(), square.clone(), kv2, table, q_out=square.transpose(1, 2))
+    got = cg.cutile_paged_kv_append(square.clone(), square, square, kv2, table)
+    x = square.clone()
+    assert torch.equal(cg.cutile_paged_kv_append(x, square, square, kv2, table, q_out=x), got)
+    one = square[:, :, :1].clone()               # the stride of a dimension of size 1 says nothing
+    want = cg.cutile_paged_kv_append(one, one, one, kv2, table)
+    x = one.clone()
+    other = torch.as_strided(x, x.shape, (x.stride(0), x.stride(1), 8, 1))
+    assert torch.equal(cg.cutile_paged_kv_append(x, one, one, kv2, table, q_out=other), want) and torch.equal(x, want)
