@@ -172,7 +172,8 @@ static int launch(Kernel kernel, const Attn& p, int phase, int splits, int two, 
     const int64_t rows = (int64_t)p.T * p.share * (phase == kPrefix ? p.per : 1);
     const int64_t ctas = (rows + 15) / 16 * splits * p.K * (phase == kPrefix ? p.B / p.per : p.B);
     const int64_t share_keys = ((int64_t)(phase == kOwn ? 0 : p.pcap) + (phase == kPrefix ? 0 : p.cap)) / splits;
-    const int fit = sizeof(T) == 4 ? 2 : 3;   // CTAs of four warps on an SM
+    constexpr int fit = Rows<T, 64, 4>::kCtas;   // CTAs of four warps on an SM
+    static_assert(fit == Rows<T, 32, 4>::kCtas && fit == Rows<T, 128, 4>::kCtas, "the same at every head size");
     a.two_warps = ctas > (int64_t)fit * device_sm_count() && share_keys <= 512;
     return launch_rows<T>(p, a, st);
   }

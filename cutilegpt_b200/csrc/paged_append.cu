@@ -171,7 +171,8 @@ static int launch_append(const Append& p, int64_t heads, cudaStream_t st) {
   const int64_t units = (p.D + 2 * V - 1) / (2 * V);
   // Two pairs of vectors a thread where that leaves threads enough to fill the GPU (8 prompts of 4093 tokens: 172 us,
   // 144 with two).
-  if (V > 1 && units % 2 == 0 && p.B * p.T * heads * units >= (1 << 20)) return launch_append_n<T, V, 2>(p, heads, units / 2, st);
+  if constexpr (V > 1)
+    if (units % 2 == 0 && (int64_t)p.B * p.T * heads * units >= (1 << 20)) return launch_append_n<T, V, 2>(p, heads, units / 2, st);
   return launch_append_n<T, V, 1>(p, heads, units, st);
 }
 

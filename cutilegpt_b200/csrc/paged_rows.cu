@@ -11,7 +11,7 @@
 // registers. S = Q Kᵀ and O += P V are tensor-core products of 16 rows
 // (mma.sync: 16 rows cannot fill the 128 rows of a tcgen05 tile; those run in paged_tc.cu).
 // No barrier stands between a warp's loads and its products; 12 to 16 warps of an
-// SM keep 96 to 128 KB in flight.
+// SM keep 96 to 144 KB in flight (fp32: 8 warps, 64 KB).
 // B200: 128 sequences of up to 4096 positions, 8 key heads of 128 in bf16 (1.08 GB): 174 us = 6.2 TB/s, 0.95 of a
 // measured copy; 67 of up to 1024: 36 us = 4.0 TB/s (the last CTAs alone). Below some 300 keys a CTA its fixed
 // chain rules (length, page table, first copies, join: about 5 us): 64 of up to 256, 12 heads of 64: 13.4 us.
@@ -39,7 +39,6 @@ struct Rows {
   // Steps of a warp's ring. Deeper ones cost resident CTAs: with four warps a fourth step pays (48 drafts of 5 tokens,
   // D = 64: 31.5 -> 30.0 us), with two it does not (64 samples of 768 + 256 positions: 13.4 us, 18.7 with four steps).
   static constexpr int kRing = kTile > 2048 ? 2 : W == 4 ? 4 : 3;
-  static constexpr int kCtas = (kWide ? 8 : DP == 128 ? 12 : 16) / W;   // of an SM
   // Q fragments in shared memory, read at every step, where they would take too many registers
   static constexpr bool kQShared = kWide || DP == 128;
   static constexpr int kQSteps = kWide ? DP / 4 : DP / 16;     // uint4 of a lane
@@ -47,6 +46,9 @@ struct Rows {
   static constexpr int kRings = W * kRing * 2 * kTile;
   static constexpr int kMerge = W * kRowTile * (DP + 2) * 4 + kRowTile * kMaxSlots * 8;
   static constexpr int kSmem = (kRings > kMerge ? kRings : kMerge) + kQ;
+  // CTAs of an SM: as many as its registers give room for (8, 12 or 16 warps), or its shared memory
+  static constexpr int kByRegs = (kWide ? 8 : DP == 128 ? 12 : 16) / W, kBySmem = 227 * 1024 / (kSmem + 1024);
+  static constexpr int kCtas = kByRegs < kBySmem ? kByRegs : kBySmem;
 };
 
 // Byte offset of 16-byte chunk c of row r in a tile of rows of DP values, chunks permuted
