@@ -156,11 +156,13 @@ def cutile_paged_kv_append(q, k, v, kv: PagedKV, cos_sin=None, interleaved: bool
         ops.paged_kv_append(None, k, v, None, kv)
         return q
     q = _rows(q, "q", kv, None, tokens)
-    table = cos_sin.shape if isinstance(cos_sin, torch.Tensor) else ()
+    if type(cos_sin) is not torch.Tensor:
+        cos_sin = as_cuda(cos_sin, "cos_sin")
+    table = cos_sin.shape
     if (len(table) != 2 or cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or table[0] == 0 or table[1] % 2
             or not 0 < table[1] <= kv.head_dim or cos_sin.device != kv.device):
         raise ValueError(f"cos_sin: expected a contiguous float32 [n_pos, rot] table with even rot <= {kv.head_dim} on "
-                         f"{kv.device}, got {getattr(cos_sin, 'dtype', type(cos_sin))} {tuple(table)}")
+                         f"{kv.device}, got {cos_sin.dtype} {tuple(table)}")
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
@@ -192,4 +194,6 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
         out = _out_rows(out, "out", kv, heads, tokens)
         if out.data_ptr() == q.data_ptr() and q.numel():
             raise ValueError("out: must not be q's memory")
+    if workspace is not None and type(workspace) is not torch.Tensor:
+        workspace = as_cuda(workspace, "workspace")
     return ops.shared_prefix_attention(q, kv, out, dim ** -0.5 if scale is None else scale, workspace)

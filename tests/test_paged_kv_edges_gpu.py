@@ -382,3 +382,16 @@ def test_outputs_in_the_way_are_refused():
     x = one.clone()
     other = torch.as_strided(x, x.shape, (x.stride(0), x.stride(1), 8, 1))
     assert torch.equal(cg.cutile_paged_kv_append(x, one, one, kv2, table, q_out=other), want) and torch.equal(x, want)
+
+
+def test_tables_and_workspaces_of_another_library():
+    kv, q = make(BF, 3, 1, 2, 4, 2, 64, 16, [900], [3, 17, 30])
+    ws = torch.empty(kv.workspace_bytes(4, 2), dtype=torch.uint8, device="cuda")
+    assert ws.numel() > 0
+    assert torch.equal(cg.cutile_shared_prefix_attention(q, kv, workspace=Producer(ws)), cg.cutile_shared_prefix_attention(q, kv))
+    k, table = torch.randn(3, 2, 2, 64, device="cuda").to(BF), torch.randn(950, 64, device="cuda")
+    want = cg.cutile_paged_kv_append(q, k, k, kv, table)
+    assert torch.equal(cg.cutile_paged_kv_append(q, k, k, kv, Producer(table)), want)
+    for bad in ([1.0, 2.0], "table", Producer(table.double())):
+        with pytest.raises(ValueError):
+            cg.cutile_paged_kv_append(q, k, k, kv, bad)
