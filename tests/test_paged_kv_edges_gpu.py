@@ -239,6 +239,65 @@ def test_fp32_largest_numbers(n, D):
         kv.v_pages[pid, :, slot] = 1.0
 
 
+# ------------------------------------------------------------------ every row beside damaged tokens
+DAMAGED = [
+    (BF, 3, 1, 4, 8, 2, 64, 16, [100], [4, 40, 77]), (F32, 3, 1, 4, 8, 2, 64, 16, [100], [4, 40, 77]),
+    (BF, 3, 1, 33, 4, 2, 64, 64, [190], [33, 40, 64]), (BF, 2, 1, 150, 4, 1, 128, 64, [260], [150, 400]),
+    (BF, 2, 0, 9, 2, 2, 128, 16, [], [9, 300]), (BF, 2, 1, 3, 2, 1, 7, 16, [20], [3, 30]),
+    (BF, 2, 1, 5, 2, 2, 64, 16, [700], [2, 30]), (F32, 2, 1, 5, 2, 2, 64, 16, [700], [2, 30]),   # padding among the rows
+]
+
+
+@pytest.mark.parametrize("what", ["values", "keys", "both"])
+@pytest.mark.parametrize("case", DAMAGED, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_every_row_beside_damaged_tokens(case, what):
+    """Two of the new tokens hold infinities and NaN: all rows, before, at and behind them, against the definition."""
+    kv, q = make(*case)
+    T, seq = case[3], case[9]
+    for pages, junk in ((kv.v_pages, (INF, -INF, NAN)), (kv.k_pages, (-INF, NAN, INF))):
+        if what != "both" and (pages is kv.v_pages) != (what == "values"):
+            continue
+        for b, n in enumerate(seq):
+            for t, x in ((T // 2, junk[0]), (T - 1, junk[1 + b % 2])):
+                i = n - T + t
+                if i >= 0:
+                    pid, slot = spot(kv, b, i)
+                    pages[pid, :, slot] = x
+    ref = check(q, kv)
+    live = [b for b, n in enumerate(seq) if n >= T]
+    assert ref[live, :, :T // 2].isfinite().all() and not ref[live, :, T - 1].isfinite().any()
+
+
+# ------------------------------------------------------------------ tables for a server's longest context
+WIDE = [
+    (BF, 4, 1, 1, 12, 12, 64, 16, [96], [1, 5, 16, 17]),
+    (BF, 67, 1, 1, 8, 2, 128, 64, [810], [i % 103 for i in range(67)]),
+    (F32, 13, 1, 1, 3, 3, 64, 16, [103], [i % 8 for i in range(13)]),
+    (BF, 48, 3, 5, 6, 2, 64, 32, [200, 33, 7], [5 + i % 50 for i in range(48)]),
+    (BF, 2, 1, 40, 8, 2, 128, 64, [300], [40, 90]), (BF, 2, 0, 3, 2, 1, 7, 16, [], [3, 30]),
+]
+
+
+@pytest.mark.parametrize("width", [1000, 65536])
+@pytest.mark.parametrize("case", WIDE, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_tables_wider_than_the_lengths(case, width):
+    """Shares, joins and launches go by the tables' width; entries behind a length are no pages and are not read."""
+    kv, q = make(*case)
+    want = cg.cutile_shared_prefix_attention(q, kv).double().cpu()
+
+    def widen(table):
+        if table is None:
+            return None
+        wide = torch.full((table.shape[0], width // case[7]), -7, dtype=torch.int32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        return wide
+
+    kv2 = cg.PagedKV(kv.k_pages, kv.v_pages, widen(kv.page_table), kv.seq_lens, widen(kv.prefix_table), kv.prefix_lens)
+    check(q, kv2)
+    ref, tol = definition(q, kv, q.shape[-1] ** -0.5)
+    assert ((want - ref).abs() <= tol).all()
+
+
 # ------------------------------------------------------------------ the range of values
 RISING = [
     # enough sequences, groups and key heads that a CTA sees several tiles
