@@ -367,6 +367,55 @@ def test_append_past_the_table(dtype, D, rot, T, past):
     assert torch.equal(got, want)
 
 
+# ------------------------------------------------------------------ steps that follow each other
+@pytest.mark.parametrize("dtype,B,T,H,K,D,prefix,own", [
+    (BF, 64, 1, 12, 12, 64, 768, 200), (BF, 60, 1, 32, 8, 128, 1100, 300), (BF, 48, 5, 24, 8, 64, 517, 130),
+    (BF, 8, 20, 8, 2, 64, 700, 200), (F32, 13, 1, 12, 12, 64, 1003, 77), (BF, 4, 1, 12, 12, 64, 96, 16),
+    (BF, 64, 1, 32, 8, 128, 33000, 2000)])
+def test_steps_back_to_back(dtype, B, T, H, K, D, prefix, own):
+    """Append and attention over and over on the same buffers, nothing between them: no step sees an earlier one's
+    queries or keys, though the launches overlap. Lengths and tables change between two rounds."""
+    steps = 24
+    kv, _ = make(dtype, B, 1, T, H, K, D, 64, [prefix], [T + (i * 7) % (own - T) for i in range(B)], garbage=False)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(steps, B, T, H + 2 * K, D, generator=g, device="cuda").to(dtype)
+    table = torch.randn(prefix + own + 64, D, generator=g, device="cuda")
+    ws = torch.empty(max(16, kv.workspace_bytes(H, T)), dtype=torch.uint8, device="cuda")
+    qbuf = torch.empty(B, H, T, D, dtype=dtype, device="cuda")
+    outs = torch.empty(steps, B, H, T, D, dtype=dtype, device="cuda")
+    lens = kv.seq_lens.clone(), kv.seq_lens.flip(0).contiguous()
+    tables = kv.page_table.clone(), kv.page_table.flip(0).contiguous()
+
+    def run(wait):
+        for i in range(steps):
+            if i % 8 == 0:
+                kv.seq_lens.copy_(lens[i // 8 % 2])
+                kv.page_table.copy_(tables[i // 8 % 2])
+            q, k, v = (y.transpose(1, 2) for y in x[i].split([H, K, K], dim=2))
+            cg.cutile_paged_kv_append(q, k, v, kv, table, q_out=qbuf)
+            if wait:
+                torch.cuda.synchronize()
+            cg.cutile_shared_prefix_attention(qbuf, kv, out=outs[i], workspace=ws)
+            if wait:
+                torch.cuda.synchronize()
+                qbuf.fill_(NAN)
+                ws.fill_(255)
+
+    pages = kv.k_pages.clone(), kv.v_pages.clone()
+    run(True)
+    want = outs.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(False)
+    for again in (lambda: run(False), graph.replay, graph.replay):
+        kv.k_pages.copy_(pages[0])
+        kv.v_pages.copy_(pages[1])
+        outs.fill_(NAN)
+        again()
+        assert torch.equal(outs, want)
+    assert L.device_error() == 0
+
+
 # ------------------------------------------------------------------ calls from several threads
 def test_attention_from_several_threads():
     """Head sizes whose tiles need different amounts of shared memory, at the same time."""
