@@ -658,6 +658,40 @@ def run_prefill_parts(local):
     print(json.dumps({"probe": "prefill_parts", "unit": "us per part sequence", "parts": out}), flush=True)
 
 
+def run_samples_probe(local):
+    """generate_samples (prompt pages shared) beside generate on the repeated prompt: one prompt of 768 tokens, 64 samples
+    of 256 tokens, top-k 50, bf16; best of three calls each (wall time, synchronised) and the memory they hold beside
+    the weights. Prints one JSON line."""
+    from cutilegpt_b200 import CutileGPT, GPTConfig
+    dev = torch.device("cuda", local)
+    torch.cuda.set_device(dev)
+    idx = torch.randint(0, 50257, (1, 768), generator=torch.Generator().manual_seed(1)).to(dev)
+    rows = idx.repeat_interleave(64, 0)
+    out = {}
+    for name, cfg in (("gpt2", GPTConfig.gpt2()), ("gpt2-xl", GPTConfig.gpt2_xl())):
+        m = CutileGPT(cfg, dtype=torch.bfloat16, device=dev, seed=0)
+        m._fold_weights()            # both use them: not counted
+        out[name] = {}
+        for what, fn in (("generate_samples", lambda: m.generate_samples(idx, 64, 256, top_k=50)),
+                         ("generate", lambda: m.generate(rows, 256, top_k=50))):
+            torch.cuda.empty_cache()
+            base = torch.cuda.memory_allocated()
+            torch.cuda.reset_peak_memory_stats()
+            fn()
+            best = math.inf
+            for _ in range(3):
+                torch.cuda.synchronize()
+                t0 = time.perf_counter()
+                fn()
+                torch.cuda.synchronize()
+                best = min(best, time.perf_counter() - t0)
+            out[name][what] = {"ms": round(best * 1e3, 1), "GB": round((torch.cuda.max_memory_allocated() - base) / 1e9, 2)}
+            for cache in (m._samples, m._dec, m._ws):
+                cache.clear()
+        del m
+    print(json.dumps({"probe": "samples", "prompt": 768, "samples": 64, "new": 256, "models": out}), flush=True)
+
+
 def run_probe(name, local):
     """One HBM-bound kernel alone, at a size whose inputs exceed the 126 MB L2, timed with CUDA events
     (3 warm-up + 10 timed launches); the profiling command runs the same probe under ncu.
@@ -732,14 +766,18 @@ def main():
     ap.add_argument("--no-cpu", action="store_true")
     ap.add_argument("--no-xl", action="store_true", help="skip the config-5 (GPT-2 XL) extras")
     ap.add_argument("--decode-only", action="store_true", help="only the config-4 decode run (profiling)")
-    ap.add_argument("--probe", choices=["layernorm", "gelu", "decode_attn", "decode_parts", "prefill_parts"], default=None,
-                    help="time one HBM-bound kernel alone at a size larger than L2 (profiling)")
+    ap.add_argument("--probe", choices=["layernorm", "gelu", "decode_attn", "decode_parts", "prefill_parts", "samples"],
+                    default=None, help="time one HBM-bound kernel alone at a size larger than L2 (profiling), the parts "
+                                       "of a step, or samples of a prompt beside generate")
     args = ap.parse_args()
     args.warmup = max(args.warmup, 3)
 
     world_env = int(os.environ.get("WORLD_SIZE", "1"))
     if args.probe == "prefill_parts":
         run_prefill_parts(int(os.environ.get("LOCAL_RANK", "0")))
+        return
+    if args.probe == "samples":
+        run_samples_probe(int(os.environ.get("LOCAL_RANK", "0")))
         return
     if args.probe == "decode_parts":
         run_decode_parts(int(os.environ.get("LOCAL_RANK", "0")))
