@@ -180,8 +180,10 @@ def cutile_shared_prefix_attention(q, kv: PagedKV, scale: float | None = None, o
     q (batch, n_head, tokens, head_dim), n_head a multiple of the cache's key heads (head h reads key head
     h // (n_head // n_kv_head)); token t of sequence b sees the prefix and its own positions 0 ..
     seq_lens[b] - tokens + t, and gives zeros where that is negative (padding, idle sequences). The prefix
-    is read once for all sequences of its group. scale is 1/√head_dim by default. A new contiguous tensor is
-    returned unless `out` (any strides, contiguous head_dim, no overlap with q) is given; `workspace` (uint8,
+    is read once for a block of its sequences' rows, 128 or 256 of a key head in bf16 with the usual sizes
+    (see the C header), not once for a sequence. In bf16 the probabilities are rounded to bf16 for their
+    product with the values. scale is 1/√head_dim by default. A new contiguous tensor is returned unless `out`
+    (any strides, contiguous head_dim, no overlap with q) is given; `workspace` (uint8,
     kv.workspace_bytes(n_head, tokens)) is allocated unless given.
     """
     q = _rows(q, "q", kv, None, None)

@@ -521,8 +521,9 @@ class CutileGPT:
 
         A prompt is prefilled once and its keys and values are kept once, in pages that all its samples
         share; each sample's own positions have pages of their own. Sample j of prompt i draws as row
-        i * num_samples + j of a batch does. Past block_size the windowed generation of `generate` runs
-        on the repeated prompts.
+        i * num_samples + j of a batch does. In bf16 the decode steps round the attention probabilities to
+        bf16, where those of `generate` keep fp32, so that logits differ by bf16 rounding; in fp32 they agree.
+        Past block_size the windowed generation of `generate` runs on the repeated prompts.
         """
         idx = self._prep_idx(idx)
         P, T0 = idx.shape

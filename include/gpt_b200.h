@@ -350,10 +350,15 @@ GPT_API int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H,
  * rows that see them and no others (where a value of a new token holds one,
  * the rows of its CTA are computed again, slowly). Weighted values are summed
  * in fp32 before the division: values near the largest number may overflow
- * where several keys share the weight. What the sequences of a group share is read once for all of them;
- * parts of the keys are computed apart and joined through `workspace`
- * (gpt_attention_shared_prefix_workspace_size bytes, 16-byte aligned; NULL
- * when that is 0). scale must be positive and finite. out must not overlap q.
+ * where several keys share the weight. In bf16 the probabilities are rounded
+ * to bf16 for the product with the values (their sum is not). A group's prefix
+ * is read once for each block of its sequences' rows (T * H / kv_heads rows a
+ * sequence and key head): 256 or 128 of them in bf16 with head_dim 64 or 128
+ * and aligned pages of a multiple of 8 positions (up to 128, or of 128), 16
+ * otherwise. Sequences with 128 rows or more, and any over a short prefix,
+ * read it by themselves. Parts of the keys are computed apart and joined
+ * through `workspace` (gpt_attention_shared_prefix_workspace_size bytes,
+ * 16-byte aligned; NULL when that is 0). scale must be positive and finite. out must not overlap q.
  * Strides as above. */
 GPT_API int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides,
                void* out, const int64_t* out_strides, int64_t T, int64_t H,
