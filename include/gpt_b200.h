@@ -358,8 +358,8 @@ GPT_API int64_t gpt_attention_shared_prefix_workspace_size(int64_t T, int64_t H,
  * otherwise. Sequences with 128 rows or more, and any over a short prefix,
  * read it by themselves. Parts of the keys are computed apart and joined
  * through `workspace` (gpt_attention_shared_prefix_workspace_size bytes,
- * 16-byte aligned; NULL when that is 0). scale must be positive and finite. out must not overlap q.
- * Strides as above. */
+ * 16-byte aligned; NULL when that is 0). scale must be positive and finite.
+ * out must not overlap q. Strides as above. */
 GPT_API int gpt_attention_shared_prefix(const void* q, const int64_t* q_strides,
                void* out, const int64_t* out_strides, int64_t T, int64_t H,
                const gpt_paged_kv* kv, float scale, void* workspace,
