@@ -11,6 +11,12 @@ namespace paged {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// A score times the scale is subtracted from the reference point in one fused operation, which does not round the
+// product, as the reference point was rounded: of a score of 2^b the two differ by up to 2^(b - 25), more than an exponential
+// can hold from about 2^32 on. From this size on the few-row kernel rounds the product first; paged_tc.cu has a size of its own.
+constexpr float kHugeScore = 1 << 20;
+__device__ __forceinline__ float scaled(float s, float scale) { return __fmul_rn(s, scale); }   // in no fused operation
+
 // What a launch of an attention kernel looks at.
 //   kPrefix  the rows of all sequences of a group against the group's prefix
 //   kOwn     the rows of one sequence against its own positions
@@ -163,7 +169,7 @@ __device__ __noinline__ void slow_row(const Attn& p, const Keys keys, int kh, co
     float s = 0.f;
     for (int c = 0; c < 4; ++c)
       if (off >= 0 && lane + 32 * c < p.D) s = fmaf(x[c], Tr<T>::to_f(((const T*)p.k)[off + lane + 32 * c]), s);
-    s = warp_sum(s) * p.scale_log2;
+    s = scaled(warp_sum(s), p.scale_log2);
     // a NaN score leaves m where it is, -inf at first: its exponential is NaN all the same
     const float to = fmaxf(m, s), a = m == -INFINITY ? 0.f : exp2f(m - to), e = s == -INFINITY ? 0.f : exp2f(s - to);
     m = to;

@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     for (int h = 0; h < 2; ++h) {
       mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
       // fp32: P is at most 1/2, so that a value near the largest number stays in range while its parts are added
-      mx[h] = fmaf(fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)), p.scale_log2, kWide ? 1.f : 0.f);
+      mx[h] = scaled(fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)), p.scale_log2) + (kWide ? 1.f : 0.f);
     }
     if (__any_sync(0xffffffffu, mx[0] > m[0] || mx[1] > m[1])) {
       float by[2];
@@ -365,11 +365,19 @@ __global__ void __launch_bounds__(W * 32, (Rows<T, DP, W>::kCtas)) paged_rows_ke
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) base[h] = m[h] == -INFINITY ? 0.f : m[h];   // a row without keys so far: every 2^(s - base) is 0
+    float unit = p.scale_log2;
+    if (__any_sync(0xffffffffu, fmaxf(fabsf(base[0]), fabsf(base[1])) > kHugeScore)) {
+      unit = 1.f;
+#pragma unroll
+      for (int i = 0; i < KS / 8; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sc[i][k] = scaled(sc[i][k], p.scale_log2);
+    }
 #pragma unroll
     for (int i = 0; i < KS / 8; ++i)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        sc[i][k] = attn_tc::ex2(fmaf(sc[i][k], p.scale_log2, -base[k >> 1]));
+        sc[i][k] = attn_tc::ex2(fmaf(sc[i][k], unit, -base[k >> 1]));
         l[k >> 1] += sc[i][k];
       }
     if constexpr (kWide) {

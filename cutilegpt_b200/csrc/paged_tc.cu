@@ -62,6 +62,7 @@ constexpr int kTcThreads = 12 * 32;      // 2 x 4 softmax warps, 2 MMA warps, K 
 constexpr int kPanel = 128 * 128;        // 128 rows of 64 bf16, 128-byte swizzled
 constexpr float kTcRescale = 8.f;        // rise of the largest score, in powers of two, from which the next tile moves m
 constexpr float kTcFar = 16.f;           // and from which the tile itself moves m and starts over; m lies this far above
+constexpr float kTcHugeScore = 1 << 30;  // from which a row is computed again
 
 template <int D>
 struct Tc {
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
           for (int k = 16; k < 128; k += 16)
 #pragma unroll
             for (int c = 0; c < 8; ++c) m8[c] = fmax3(m8[c], __uint_as_float(s[k + c]), __uint_as_float(s[k + 8 + c]));
-          return fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])) * p.scale_log2;
+          return scaled(fmax3(fmax3(m8[0], m8[1], m8[2]), fmax3(m8[3], m8[4], m8[5]), fmaxf(m8[6], m8[7])), p.scale_log2);
         };
         bool rescale = false;
         float alpha = 1.f;
@@ -445,31 +446,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       if (ok && !mbar_wait(smem_addr(&pb[5]), C::kAlias ? 0u : (uint32_t)((g - 1) & 1))) ok = false;
       tc_fence_after();
     }
+    // Row rr of the phase once more, key by key, by this warp.
+    auto compute_again = [&](int rr) {
+      const int te = t0 + n_tiles;
+      const int j0 = t0 < nt_pre ? t0 * a.tile : keys.n_pre + (t0 - nt_pre) * a.tile;
+      const int j1 = te <= nt_pre ? min(keys.n_pre, te * a.tile) : keys.n_pre + min(n_own, (te - nt_pre) * a.tile);
+      const Row to(p, b0, kh, rr);
+      const int end = keys.n_own - p.T + to.t;
+      float rm, rls, acc[4];
+      slow_row<__nv_bfloat16>(p, keys, kh, (const __nv_bfloat16*)p.q + to.b * p.q_b + to.h * p.q_h + to.t * p.q_t, j0,
+                              a.phase == kPrefix ? j1 : end < 0 ? j0 : min(j1, keys.n_pre + end + 1), lane, rm, rls, acc);
+      const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to.b, to.t, to.h);
+      if (!a.direct && lane == 0) p.ml[at] = make_float2(rm, rls);
+      for (int c = 0; c < D / 32; ++c) {
+        if (a.direct)
+          ((__nv_bfloat16*)p.out)[to.b * p.o_b + to.h * p.o_h + to.t * p.o_t + lane + 32 * c] =
+              __float2bfloat16_rn(end < 0 ? 0.f : acc[c] / rls);
+        else if (rls != 0.f)
+          p.acc[at * D + lane + 32 * c] = acc[c];
+      }
+    };
     bool done = false;
     if constexpr (kEdge) {
       asm volatile("bar.sync 2, 288;" ::: "memory");
       done = *again != 0;
-      if (done) {   // an infinity or NaN at the causal edge: the block's rows once more, a warp for each
+      if (done) {   // an infinity or NaN at the causal edge: the block's rows, a warp for each
         if (a.early) pdl_wait();
-        const int te = t0 + n_tiles;
-        const int j0 = t0 < nt_pre ? t0 * a.tile : keys.n_pre + (t0 - nt_pre) * a.tile;
-        const int j1 = te <= nt_pre ? min(keys.n_pre, te * a.tile) : keys.n_pre + min(n_own, (te - nt_pre) * a.tile);
-        for (int rr = r0 + warp; rr < min(rows, r0 + (a.two ? 256 : 128)); rr += 8) {
-          const Row to(p, b0, kh, rr);
-          const int end = keys.n_own - p.T + to.t;
-          float rm, rls, acc[4];
-          slow_row<__nv_bfloat16>(p, keys, kh, (const __nv_bfloat16*)p.q + to.b * p.q_b + to.h * p.q_h + to.t * p.q_t, j0,
-                                  end < 0 ? j0 : min(j1, keys.n_pre + end + 1), lane, rm, rls, acc);
-          const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to.b, to.t, to.h);
-          if (!a.direct && lane == 0) p.ml[at] = make_float2(rm, rls);
-          for (int c = 0; c < D / 32; ++c) {
-            if (a.direct)
-              ((__nv_bfloat16*)p.out)[to.b * p.o_b + to.h * p.o_h + to.t * p.o_t + lane + 32 * c] =
-                  __float2bfloat16_rn(end < 0 ? 0.f : acc[c] / rls);
-            else if (rls != 0.f)
-              p.acc[at * D + lane + 32 * c] = acc[c];
-          }
-        }
+        for (int rr = r0 + warp; rr < min(rows, r0 + (a.two ? 256 : 128)); rr += 8) compute_again(rr);
       }
     }
     // The row's result: out, or its slot of partial results. Two pipelines on the same rows see each
@@ -489,9 +492,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) paged_tc_kernel(const __grid_co
       m = to;
     }
     if (a.early) pdl_wait();
+    // Scores of 2^30 and more lose more in the fused operation (see kHugeScore) than the 2^16 between 1 and P can make
+    // up for. Looking for them in every tile costs 1 to 4%: such rows are computed again.
+    const bool huge = live && pipe < pipes && fabsf(m) > kTcHugeScore && !isinf(m);
+    if (const uint32_t rest = __ballot_sync(0xffffffffu, huge); rest && !done && (a.two || pipe == 0))
+      for (uint32_t left = rest; left; left &= left - 1) compute_again(r - lane + __ffs(left) - 1);
     const Row to_row(p, b0, kh, live ? r : r0);
     const int64_t at = ((int64_t)a.slot0 + split) * p.B * p.T * p.H + row_id(p, to_row.b, to_row.t, to_row.h);
-    const bool mine = live && !done && (a.two || shared_rows || pipe == 0), none = l == 0.f;
+    const bool mine = live && !done && !huge && (a.two || shared_rows || pipe == 0), none = l == 0.f;
     const uint32_t no_keys = last < 0 ? 0u : 0x7fc07fc0u;   // zeros for padding, else every score is -inf: 0 / 0
     if (mine && !a.direct && (a.two || pipe == 0)) p.ml[at] = make_float2(m, l);
     if (a.direct) {

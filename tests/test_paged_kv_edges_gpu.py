@@ -239,6 +239,38 @@ def test_fp32_largest_numbers(n, D):
         kv.v_pages[pid, :, slot] = 1.0
 
 
+# ------------------------------------------------------------------ huge scores
+RISING = [
+    # enough sequences, groups and key heads that a CTA sees several tiles
+    (BF, 40, 0, 17, 2, 2, 64, 64, [], [700 - i for i in range(40)]),
+    (BF, 40, 0, 17, 2, 2, 128, 64, [], [700 - i for i in range(40)]),
+    (BF, 40, 0, 17, 16, 2, 64, 64, [], [450 - i for i in range(40)]),        # 256 rows on the same tiles
+    (BF, 40, 0, 17, 16, 2, 128, 64, [], [450 - i for i in range(40)]),
+    (BF, 80, 40, 1, 18, 2, 64, 64, [600] * 40, [1 + i % 5 for i in range(80)]),
+    (BF, 4, 1, 1, 2, 2, 64, 16, [517], [1, 2, 40, 300]),                     # the few-row kernel
+]
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("exponent", [20, 35, 60, 110])
+@pytest.mark.parametrize("case", ALL_KERNELS + RISING[1:5:3], ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
+def test_huge_scores(case, exponent, sign):
+    """Scores of 7 to 11 times 2^exponent, all exact: the keys with the largest share the weight, whatever its size."""
+    kv, q = make(*case)
+    q = torch.zeros_like(q)
+    q[..., 0] = sign * 2.0 ** (exponent // 2)
+    level = torch.arange(kv.k_pages[..., 0].numel(), device="cuda").view(kv.k_pages.shape[:3]) * 7 % 11 % 5 + 7
+    kv.k_pages[..., 0] = level * 2.0 ** (exponent - exponent // 2)
+    kv.k_pages[..., 1:] = 0.0
+    for scale in (0.3, 0.123, 0.0717):
+        assert check(q, kv, scale).isfinite().all()
+    if case[3] > 1:                                          # rows that are computed again
+        for b, n in enumerate(case[9]):
+            pid, slot = spot(kv, b, n - 1)
+            kv.v_pages[pid, :, slot] = INF
+        check(q, kv, 0.123)
+
+
 # ------------------------------------------------------------------ every row beside damaged tokens
 DAMAGED = [
     (BF, 3, 1, 4, 8, 2, 64, 16, [100], [4, 40, 77]), (F32, 3, 1, 4, 8, 2, 64, 16, [100], [4, 40, 77]),
@@ -299,17 +331,6 @@ def test_tables_wider_than_the_lengths(case, width):
 
 
 # ------------------------------------------------------------------ the range of values
-RISING = [
-    # enough sequences, groups and key heads that a CTA sees several tiles
-    (BF, 40, 0, 17, 2, 2, 64, 64, [], [700 - i for i in range(40)]),
-    (BF, 40, 0, 17, 2, 2, 128, 64, [], [700 - i for i in range(40)]),
-    (BF, 40, 0, 17, 16, 2, 64, 64, [], [450 - i for i in range(40)]),        # 256 rows on the same tiles
-    (BF, 40, 0, 17, 16, 2, 128, 64, [], [450 - i for i in range(40)]),
-    (BF, 80, 40, 1, 18, 2, 64, 64, [600] * 40, [1 + i % 5 for i in range(80)]),
-    (BF, 4, 1, 1, 2, 2, 64, 16, [517], [1, 2, 40, 300]),                     # the few-row kernel
-]
-
-
 @pytest.mark.parametrize("exponent", [100, -100])
 @pytest.mark.parametrize("case", RISING, ids=lambda c: "-".join(str(x) for x in (str(c[0])[6:],) + c[1:8]))
 def test_large_values_behind_rising_scores(case, exponent):
