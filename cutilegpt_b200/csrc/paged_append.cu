@@ -4,7 +4,7 @@
 // (x0 c - x1 s, x0 s + x1 c) with c, s from the caller's fp32 table; values
 // are copied. Everything is read once and written once, so the kernel is
 // bound by HBM: 2 (2 K + H) D e bytes per token with rotation, 4 K D e without.
-// B200: 8 prompts of 4093 tokens, 32 + 2 x 8 heads of 128 in bf16 (806 MB), 138.5 us = 5.8 TB/s, 0.89 of
+// B200: 8 prompts of 4093 tokens, 32 + 2 x 8 heads of 128 in bf16 (806 MB), 138.6 us = 5.8 TB/s, 0.89 of
 // a measured copy; 5 x 1021 tokens, 3 x 25 heads of 64 in fp32, 33.1 us = 5.9 TB/s; a step of 256 sequences 3.1 us.
 //
 // One thread handles two vectors of V elements of one head (16 bytes each

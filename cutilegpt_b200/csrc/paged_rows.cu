@@ -12,16 +12,16 @@
 // (mma.sync: 16 rows cannot fill the 128 rows of a tcgen05 tile; those run in paged_tc.cu).
 // No barrier stands between a warp's loads and its products; 12 to 16 warps of an
 // SM keep 96 to 144 KB in flight (fp32: 8 warps, 64 KB).
-// B200: 128 sequences of up to 4096 positions, 8 key heads of 128 in bf16 (1.08 GB): 172 us = 6.3 TB/s, 0.97 of a
+// B200: 128 sequences of up to 4096 positions, 8 key heads of 128 in bf16 (1.08 GB): 173 us = 6.2 TB/s, 0.96 of a
 // measured copy; 67 of up to 1024: 36 us = 4.1 TB/s (the last CTAs alone). Below some 300 keys a CTA its fixed
-// chain rules (length, page table, first copies, join: about 5 us): 64 of up to 256, 12 heads of 64: 13.1 us.
+// chain rules (length, page table, first copies, join: about 5 us): 64 of up to 256, 12 heads of 64: 13.2 us.
 //
 // bf16: m16n8k16. P is rounded to bf16 for its product with V, its sum is taken before.
 // fp32: m16n8k8 on TF32 parts. A value x is hi + lo, hi = x to 11 bits, lo = (x - hi) to
 // 11 bits: x is met to 2^-22, and hi hi + hi lo + lo hi leaves out 2^-22 of a product. The tensor cores
 // cut sums off towards zero, so a product chain is short (16 elements of a score, a step's keys of
 // the output) and is added to the running sum by a rounding add (13 samples of 1003 + 77 positions against
-// 64 bits: 1.2e-6 off with chains through, 4.2e-7 so). The order of a contraction is free, so a lane's operands are
+// 64 bits: 1.2e-6 off with chains through, 4.5e-7 so). The order of a contraction is free, so a lane's operands are
 // those that one 16-byte read gives it.
 #include "paged.cuh"
 

@@ -1,7 +1,7 @@
 // Attention over the paged cache on the CUDA cores, in fp32: any head size up
 // to 256, any page size, strides and alignment, both types. It serves what the tensor-core kernels'
 // conditions leave over (13 sequences behind 1003 positions, 12 heads of 64 in fp32, in views at odd
-// elements: 98 us a call; aligned, in the few-row kernel, 12.1).
+// elements: 98 us a call; aligned, in the few-row kernel, 12.0).
 //
 // A CTA of four warps takes up to RB rows of one key head (see Phase in
 // paged.cuh) and one of `splits` equal shares of the phase's keys, 32 keys a

@@ -26,7 +26,7 @@
 // Keys and values have separate rings; every wait is bounded.
 // Bound by the softmax warps' issue: a pair of 128 x 128 tiles at D = 128 takes 4300 clocks, of which the products
 // and the special-function unit need 2048 each. B200: 8 questions of 256 tokens behind 4096 + 700 positions, 32 heads
-// (149 GFLOP): 173 us = 863 TF/s; 512 rows of each of 8 key heads against 65536 keys: 148 to 164 us = 838 to 928 TF/s.
+// (149 GFLOP): 175 us = 853 TF/s; 512 rows of each of 8 key heads against 65536 keys: 148 to 162 us = 851 to 926 TF/s.
 #include "paged.cuh"
 
 namespace gpt {
